@@ -311,9 +311,6 @@ def prepare(case, seed):
         s.logits, s.scores, s.done = s.put(i["logits"]), s.put(i["scores"]), s.put(i["done"])
         found = c["groups"] * c["select"]
         s.parents, s.tokens, s.best = s.new(found), s.new(found), s.new(found)
-        shape = (c["groups"], c["select"])
-        s.results = {"parents": view(s.parents, *shape, dtype=torch.int32),
-                     "tokens": view(s.tokens, *shape, dtype=torch.int32), "scores": view(s.best, *shape)}
         s.i = None
     else:
         dtype = hip.DT_F32 if c["dtype"] == "f32" else hip.DT_BF16
@@ -326,9 +323,6 @@ def prepare(case, seed):
                                      share=c["share"])
             s.parents, s.tables, s.history = s.put(i["parents"]), s.new(i["tables"].numel()), s.put(i["history"])
             s.new_history = s.new(i["history"].numel())
-            s.results = {"tables": view(s.tables, c["sequences"], -1, dtype=torch.int32),
-                         "history": view(s.new_history, c["sequences"], -1, dtype=torch.int32),
-                         "caches": [view(p.pages, -1, dtype=DTYPES[c["dtype"]]) for p in s.caches]}
             s.i = None
         else:
             s.cache = make(i["cache"])
@@ -340,12 +334,9 @@ def prepare(case, seed):
             s.batch = hip.PagedBatch(tables, lengths, c["sequences"], i["rows"], i["tables"].shape[1], starts=starts,
                                      share=c["share"], **prefix)
             s.q, s.out = s.put(i["q"]), s.new(i["q"].numel())
-            shape = (i["rows"], c["heads"], c["dim"])
-            s.results = {"out": view(s.out, *shape)}
             if f == "append":
                 s.k, s.v = s.put(i["k"]), s.put(i["v"])
-                s.results = {"q": view(s.out, *shape), "cache": view(s.cache.pages, -1, dtype=DTYPES[c["dtype"]])}
-            s.i = None
+            s.i = dict(rows=i["rows"])
     torch.cuda.synchronize()
     context().Flush()
     return s
@@ -362,14 +353,20 @@ def run(s):
     if f == "select":
         ctx.BeamSelect(s.parents, s.tokens, s.best, s.logits, s.scores, s.done, c["groups"], c["beams"], c["vocab"],
                        c["select"], 2)
-    elif f == "reorder":
+        shape = (c["groups"], c["select"])
+        return {"parents": view(s.parents, *shape, dtype=torch.int32), "tokens": view(s.tokens, *shape, dtype=torch.int32),
+                "scores": view(s.best, *shape)}
+    if f == "reorder":
         ctx.PagedReorder(s.batch, s.tables, s.parents, s.caches)
         ctx.GatherRows(s.new_history, s.history, s.parents, c["sequences"], c["history"])
-    elif f == "append":
+        return {"tables": view(s.tables, c["sequences"], -1, dtype=torch.int32),
+                "history": view(s.new_history, c["sequences"], -1, dtype=torch.int32),
+                "caches": [view(p.pages, -1, dtype=DTYPES[c["dtype"]]) for p in s.caches]}
+    if f == "append":
         ctx.PagedAppend(s.cache, s.batch, s.k, s.v, s.q, s.out, c["heads"], THETA)
-    else:
-        ctx.PagedAttention(s.out, s.q, s.cache, s.batch, c["heads"], c["window"], c["softcap"])
-    return s.results  # the context's tensors, as torch sees them
+        return {"q": view(s.out, -1, c["heads"], c["dim"]), "cache": view(s.cache.pages, -1, dtype=DTYPES[c["dtype"]])}
+    ctx.PagedAttention(s.out, s.q, s.cache, s.batch, c["heads"], c["window"], c["softcap"])
+    return {"out": view(s.out, -1, c["heads"], c["dim"])}
 
 
 # ---- plain forms ------------------------------------------------------------------------------------------------
