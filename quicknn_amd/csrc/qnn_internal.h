@@ -23,8 +23,12 @@ struct Error : std::runtime_error {
   Error(int c, const std::string &m) : std::runtime_error(m), code(c) {}
 };
 [[noreturn]] inline void fail(int code, const std::string &msg) { throw Error(code, msg); }
+// The runtime's record of the error is cleared: it is reported here, and the
+// check behind the next launch shall not report it again.
 inline void hip_check(hipError_t e, const char *what) {
-  if (e != hipSuccess) fail(QNN_E_INVALID_OP, std::string(what) + ": " + hipGetErrorString(e));
+  if (e == hipSuccess) return;
+  (void)hipGetLastError();
+  fail(QNN_E_INVALID_OP, std::string(what) + ": " + hipGetErrorString(e));
 }
 // a + b*c with the product rounded before the sum (never fused into an fma):
 // the accumulate of moe.comp:70 / :126 as the reference's CPU path computes it.

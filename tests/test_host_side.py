@@ -1,0 +1,74 @@
+"""The library's host side on a machine without a GPU: its calls run against a stand-in for the HIP runtime
+(hip_recorder.cpp), which keeps device memory in host memory, counts kernels instead of running them, and can make an
+allocation fail.  Each test is a process of its own, so that the library resolves to the stand-in."""
+import os
+import subprocess
+import sys
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+PRELUDE = """
+import ctypes, sys
+import numpy as np
+rec = ctypes.CDLL({stub!r}, ctypes.RTLD_GLOBAL)
+for n in ("allocations", "live_bytes", "largest"):
+    getattr(rec, "rec_" + n).restype = ctypes.c_uint64
+rec.rec_fail_at.argtypes = [ctypes.c_int64]
+rec.rec_launched.restype = ctypes.c_char_p
+from quicknn_amd import hip
+
+def raises(kind, f, *a, **kw):
+    try:
+        f(*a, **kw)
+    except kind as e:
+        return str(e)
+    raise AssertionError((kind, a, kw))
+
+ctx = hip.GPUContext(0)
+"""
+
+
+@pytest.fixture(scope="module")
+def host(tmp_path_factory):
+    """host(code): runs it with `hip`, a context `ctx` and the stand-in `rec`."""
+    stub = str(tmp_path_factory.mktemp("rec") / "libhip_recorder.so")
+    subprocess.run(["g++", "-O1", "-std=c++17", "-shared", "-fPIC", os.path.join(ROOT, "tests", "hip_recorder.cpp"), "-o",
+                    stub], check=True)
+
+    def run(code):
+        r = subprocess.run([sys.executable, "-c", PRELUDE.format(stub=stub) + code], cwd=ROOT, capture_output=True, text=True,
+                           timeout=120)
+        assert r.returncode == 0, r.stdout + r.stderr
+
+    return run
+
+
+GROW = """
+def int4(n, k):
+    w = hip.MemoryBlock.int4(np.zeros((n, (k + 31) // 32 * 20), np.uint8))
+    ctx.RetainWeight(w, n, w.shape[1])
+    return w
+
+def linear(w, k, n):
+    ctx.Int4Linear(y, x, w, 1, k, n)
+
+small, large = int4(64, 4096), int4(4096, 9728)
+x, y = ctx.NewTensor(9728), ctx.NewTensor(4096)
+linear(small, 4096, 64)
+ctx.Flush()
+"""
+
+
+def test_an_error_is_reported_once(host):
+    """A failed allocation is that call's error, not the next launch's too."""
+    host(GROW + """
+logits, scores, found = ctx.NewTensor(8000), ctx.NewTensor(4), [ctx.NewTensor(4) for _ in range(3)]
+rec.rec_fail_at(0)
+assert "out of memory" in raises(hip.EInvalidOp, ctx.BeamSelect, *found, logits, scores, None, 1, 4, 2000, 4)
+rec.rec_forget_launched()
+linear(small, 4096, 64)
+ctx.BeamSelect(*found, logits, scores, None, 1, 4, 2000, 4)
+ctx.Flush()
+assert rec.rec_launched().count(b"k_beam") == 2 and rec.rec_launched().count(b"\\n") == 3
+""")
