@@ -288,8 +288,13 @@ void ensure_splitk(qnn_ctx_s *ctx, size_t partial_floats, size_t counters) {
   retire(ctx, ctx->counters);
   ctx->partial = nullptr;
   ctx->counters = nullptr;
+  ctx->partial_floats = ctx->counter_count = 0;  // until both are there again
   hip_check(hipMalloc(&ctx->partial, std::max<size_t>(partial_floats, 1) * 4), "workspace allocation");
-  hip_check(hipMalloc(&ctx->counters, std::max<size_t>(counters, 1) * 4), "workspace allocation");
+  if (const hipError_t e = hipMalloc(&ctx->counters, std::max<size_t>(counters, 1) * 4); e != hipSuccess) {
+    (void)hipFree(ctx->partial);
+    ctx->partial = nullptr;
+    hip_check(e, "workspace allocation");
+  }
   // On the context stream and waited for: a plain hipMemset runs on the null
   // stream, which a non-blocking stream does not wait for, so the next kernel
   // could read tickets left in the recycled allocation.

@@ -72,3 +72,19 @@ ctx.BeamSelect(*found, logits, scores, None, 1, 4, 2000, 4)
 ctx.Flush()
 assert rec.rec_launched().count(b"k_beam") == 2 and rec.rec_launched().count(b"\\n") == 3
 """)
+
+
+@pytest.mark.parametrize("which", [0, 1])
+def test_a_failed_workspace_leaves_none_behind(host, which):
+    """When one of the split-K workspace's two allocations fails, the next call makes a workspace of its own instead of
+    taking the one that is gone for there, and the other allocation is not lost."""
+    host(GROW + f"""
+rec.rec_fail_at({which})
+assert "out of memory" in raises(hip.EInvalidOp, linear, large, 9728, 4096)
+before = rec.rec_allocations()
+linear(small, 4096, 64)
+assert rec.rec_allocations() == before + 2
+linear(large, 9728, 4096)
+ctx.close()
+assert rec.rec_live_bytes() == 0
+""")
