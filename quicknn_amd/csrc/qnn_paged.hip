@@ -33,6 +33,19 @@ __device__ __forceinline__ int row_sequence(const PagedBatch &b, int row) {
   return lo;
 }
 
+// The searches for a row's or group's sequence meet only some sequences where
+// row starts do not ascend, and none without rows: with row starts, every
+// sequence's data are looked at here, spread over the launch.
+__device__ __forceinline__ void report_batch(const PagedBatch &b) {
+  if (!b.starts || blockIdx.y) return;
+  for (int s = blockIdx.x * kAppendThreads + threadIdx.x; s < b.sequences; s += gridDim.x * kAppendThreads) {
+    int first, end;
+    dev::row_range(b, s, first, end);
+    dev::own_length(b, s);
+    dev::prefix_length(b, s / b.share);
+  }
+}
+
 template <int E, typename T>
 __global__ __launch_bounds__(kAppendThreads) void k_paged_append(const PagedCache c, const PagedBatch b, const float *k,
                                                                  const float *v, const float *q, float *q_out, int heads,
@@ -40,6 +53,7 @@ __global__ __launch_bounds__(kAppendThreads) void k_paged_append(const PagedCach
 #pragma clang fp contract(off)
   __shared__ double cs[kAppendMaxDim / 2], sn[kAppendMaxDim / 2];
   const int row = blockIdx.x, dim = c.dim, half = dim / 2, tid = threadIdx.x;
+  report_batch(b);
   const int s = row_sequence(b, row);
   if (s < 0) return;
   int first, end;
@@ -114,6 +128,7 @@ __global__ __launch_bounds__(kAppendThreads) void k_paged_append_groups(const Pa
 #pragma clang fp contract(off)
   extern __shared__ double2 turn[];  // [32 tokens][dim / 2]
   const int id = blockIdx.x, dim = c.dim, half = dim / 2, tid = threadIdx.x;
+  report_batch(b);
   int s = 0;
   for (int step = 1 << 16; step; step >>= 1)  // the last sequence whose first group is not behind this one
     if (s + step < b.sequences && first_group(b, s + step) <= id) s += step;

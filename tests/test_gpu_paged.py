@@ -696,3 +696,28 @@ def test_bad_device_data_is_reported(ctx, rng):
         ctx.Download(dst)
     assert ctx.Download(dst, dtype=np.int32).tolist() == [0, 1, 2, 3] + [0] * 8
     free(ctx, cache, c2, new, src, idx, dst, q, k, v, out)
+
+
+@pytest.mark.parametrize("starts,own,prefix", [
+    ([0, 100, 5, 200], [256, 256, 256], None),  # groups of 32 tokens: the second sequence is behind no row and no group
+    ([0, 64, 0, 128], [256, 256, 256], None),
+    ([0, 3, 1, 4], [9, 9, 9], None),  # workgroups per row
+    ([0, 2, 2, 1, 2], [9, 9, 9, 9], None),
+    ([0, 2, 100], [9, 9], None),  # a last range wholly behind the rows
+    ([0, 1, 1, 2], [9, 1 << 20, 9], None),  # lengths of sequences without rows
+    ([0, 1, 1, 2], [9, -1, 9], None),
+    ([0, 70, 70], [90, 1 << 20], None),
+    ([0, 1, 1], [9, 9], [5, 1 << 20])])
+def test_append_reports_what_no_row_leads_to(ctx, rng, starts, own, prefix):
+    """Row starts and lengths outside their range are reported wherever they stand in the batch."""
+    page, kv, heads, dim = 64, 1, 2, 32
+    batch = Batch(rng, page, [1] * len(own), [256] * len(own), None if prefix is None else [64] * len(own))
+    store = Store(rng, BF16, batch.pages, page, kv, dim)
+    batch.rows, batch.prefix = min(starts[-1], 2) if starts[-1] == 100 else starts[-1], prefix or batch.prefix
+    cache, b = store.put(ctx), batch.put(ctx, lengths=own, starts=starts)
+    q, k, v = (up(ctx, rng.standard_normal(batch.rows * h * dim).astype(np.float32)) for h in (heads, kv, kv))
+    ctx.PagedAppend(cache, b, k, v, q, q, heads, THETA)
+    with pytest.raises(hip.EInvalidOp, match="outside its range"):
+        ctx.Download(q)
+    ctx.Download(q)
+    free(ctx, cache, b, q, k, v)
