@@ -159,11 +159,12 @@ __device__ __forceinline__ bool parts_of(const Args &g, const Owner &w, int o, i
   const Line line = *g.head[C];
   const unsigned share = max(line.share, 1), at = unsigned(max(g.table[C][id] + h * padded<CT>(line, units), 0));
   const int last = g.workers - 1, w0 = min(int(at / share), last);
+  const int64_t slot = int64_t(g.cols[C]) * (g.a.c.dim + 4);
   p.n = min(int((at + units - 1) / share), last) - w0 + 1;
-  p.step = int64_t(g.cols[C]) * (g.a.c.dim + 4);
-  p.first = g.parts[C] + part_slot(g, w0, int64_t(id) * g.a.c.kv_heads + h, false) * p.step +
-            size_t(c % CT) * (g.a.c.dim + 4);
-  p.rest = p.first + p.step;
+  p.first = p.n == 1 ? whole_part(g, w.prefix_group >= 0, h, int64_t(w.first) * g.group + c)
+                     : split_part(g, C, w0, false) + size_t(c % CT) * (g.a.c.dim + 4);
+  p.rest = p.first + slot;  // the next worker's first slot
+  p.step = 2 * slot;
   return p.n > 1 || w.prefix > 0;
 }
 

@@ -88,3 +88,26 @@ linear(large, 9728, 4096)
 ctx.close()
 assert rec.rec_live_bytes() == 0
 """)
+
+
+@pytest.mark.parametrize("count,share,heads,kv,dim,rows", [
+    (4096, 32, 32, 8, 128, 1), (1000, 1000, 32, 8, 128, 1), (20000, 20000, 32, 8, 128, 1), (512, 8, 64, 2, 128, 1),
+    (300, 300, 16, 2, 256, 3), (2000, 50, 8, 8, 64, 2), (8, 8, 32, 8, 128, 700)])
+def test_attention_workspace_behind_prefixes(host, count, share, heads, kv, dim, rows):
+    """With prefixes the workspace holds, for every column, one part of its own keys and one of its prefix, what each
+    of the 512 workgroups of either kind of tile leaves of split items (two parts, of 32 and 128 columns), and tables."""
+    host(f"""
+n, rows = {count}, {count * rows}
+cache = hip.PagedCache(ctx.NewTensor(hip.PagedCache.words(hip.DT_BF16, 4, 64, {kv}, {dim})), hip.DT_BF16, 4, 64, {kv}, {dim})
+starts = None if rows == n else ctx.NewTensor(n + 1)
+batch = hip.PagedBatch(ctx.NewTensor(n), ctx.NewTensor(n), n, rows, 1, starts=starts,
+                       prefix_tables=ctx.NewTensor(n // {share} * 200), prefix_lengths=ctx.NewTensor(n // {share}),
+                       prefix_pages=200, share={share})
+q, out = ctx.NewTensor(rows * {heads * dim}), ctx.NewTensor(rows * {heads * dim})
+rec.rec_forget_largest()
+before = rec.rec_allocations()
+ctx.PagedAttention(out, q, cache, batch, {heads})
+assert rec.rec_allocations() == before + 1
+column = 4 * ({dim} + 4)
+assert rec.rec_largest() <= (2 * rows * {heads} + 2 * 512 * (32 + 128)) * column + (1 << 20), rec.rec_largest()
+""")
