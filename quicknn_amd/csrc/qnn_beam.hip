@@ -76,8 +76,6 @@ struct Merge {
   unsigned key[kList];
   double value[kList];
   unsigned flat[kList];
-  double best_value[kMergeThreads / 64];
-  unsigned best_flat[kMergeThreads / 64];
 };
 
 template <int OFF>
@@ -240,55 +238,71 @@ __global__ __launch_bounds__(kMergeThreads) void k_beam_merge(const BeamArgs a, 
     a.tokens[at] = int(flat % unsigned(a.vocab));
     a.best[at] = float(c);
   };
-  int ranked = min(found, a.select);
-  if (found <= 512) {
-    if (tid < found) {
-      const double c = sh.value[tid];
-      const unsigned f = sh.flat[tid];
-      int rank = 0;
-      for (int j = 0; j < found; ++j) rank += before(sh.value[j], sh.flat[j], c, f);
-      if (rank < a.select) put(rank, c, f);
-    }
-  } else {
-    // Many (ties, or few tiles): a round per rank takes the best one behind the
-    // last, from the list or, if that ran over, from all that reach T.
-    double last_c = INFINITY;
-    unsigned last_f = 0;
+  int ranked = min(found, a.select), entries = found;
+  if (found > 512) {
+    // Many (ties, flat or masked logits, few tiles): one more pass, from the
+    // list or, if that ran over, over all that reach T.  Every wave keeps the
+    // best 64 of its share, one per lane in order; their lists are ranked below.
     ranked = a.select;
-    for (int rank = 0; rank < a.select; ++rank) {
-      double c = -INFINITY;
-      unsigned f = ~0u;
-      auto offer = [&](double c1, unsigned f1) {
-        if ((rank == 0 || before(last_c, last_f, c1, f1)) && before(c1, f1, c, f)) c = c1, f = f1;
-      };
-      if (found <= kList)
-        for (int j = tid; j < found; j += kMergeThreads) offer(sh.value[j], sh.flat[j]);
-      else
-        for (int i = wave; i < n; i += kMergeThreads / 64) {
-          if (best_of(i) < limit) continue;
-          const int b = i / tiles, t = i - b * tiles;
-          for (int j = 0; j < per_lane; ++j) {
-            const int v = sh.kind[b] == kDone ? (j == 0 && lane == 0 ? a.end : a.vocab) : t * span + j * 64 + lane;
-            const double c1 = value_of(b, v);
-            if (reaches(c1)) offer(c1, unsigned(b) * a.vocab + v);
-          }
-        }
-      for (int o = 32; o; o >>= 1) {
-        const double c1 = __shfl_xor(c, o);
-        const unsigned f1 = __shfl_xor(f, o);
-        if (before(c1, f1, c, f)) c = c1, f = f1;
+    entries = a.select * (kMergeThreads / 64);
+    double c = -INFINITY;
+    unsigned f = ~0u;
+    auto offer = [&](double c1, unsigned f1) {  // a candidate per lane, minus infinity for none
+      const double cw = __shfl(c, a.select - 1);
+      const unsigned fw = __shfl(f, a.select - 1);
+      uint64_t in = __ballot(c1 > -INFINITY && before(c1, f1, cw, fw));
+      for (; in; in &= in - 1) {
+        const int from = __ffsll(static_cast<unsigned long long>(in)) - 1;
+        const double c2 = __shfl(c1, from), above_c = __shfl_up(c, 1);
+        const unsigned f2 = __shfl(f1, from), above_f = __shfl_up(f, 1);
+        const int at = __popcll(__ballot(before(c, f, c2, f2)));
+        if (lane > at) c = above_c, f = above_f;
+        else if (lane == at) c = c2, f = f2;
       }
-      __syncthreads();
-      if (lane == 0) sh.best_value[wave] = c, sh.best_flat[wave] = f;
-      __syncthreads();
-      c = sh.best_value[0];
-      f = sh.best_flat[0];
-      for (int w = 1; w < kMergeThreads / 64; ++w)
-        if (before(sh.best_value[w], sh.best_flat[w], c, f)) c = sh.best_value[w], f = sh.best_flat[w];
-      if (tid == 0) put(rank, c, f);
-      last_c = c;
-      last_f = f;
+    };
+    auto offer_tile = [&](int i) {
+      const int b = i / tiles, t = i - b * tiles;
+      if (sh.kind[b] == kDone) {
+        offer(lane == 0 ? sh.score[b] : -INFINITY, unsigned(b) * a.vocab + a.end);
+        return;
+      }
+      const float *row = a.logits + size_t(first + b) * a.vocab;
+      for (int j0 = 0; j0 < per_lane; j0 += 8) {
+        float y[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[j] = row[min(t * span + min(j0 + j, per_lane - 1) * 64 + lane, a.vocab - 1)];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int v = t * span + (j0 + j) * 64 + lane;
+          const double c1 = j0 + j < per_lane && v < a.vocab ? candidate(b, y[j]) : -INFINITY;
+          offer(reaches(c1) ? c1 : -INFINITY, unsigned(b) * a.vocab + v);
+        }
+      }
+    };
+    if (found <= kList) {
+      for (int j0 = wave * 64; j0 < found; j0 += kMergeThreads) {
+        const int j = min(j0 + lane, found - 1);
+        offer(j0 + lane < found ? sh.value[j] : -INFINITY, sh.flat[j]);
+      }
+    } else if (count <= kList) {
+      for (int x = wave; x < count; x += kMergeThreads / 64) offer_tile(sh.list[x]);
+    } else {
+      for (int i = wave; i < n; i += kMergeThreads / 64)
+        if (best_of(i) >= limit) offer_tile(i);
     }
+    __syncthreads();  // the lists have been read
+    if (lane < a.select) {
+      sh.value[wave * a.select + lane] = c;
+      sh.flat[wave * a.select + lane] = f;
+    }
+    __syncthreads();
+  }
+  if (tid < entries) {
+    const double c = sh.value[tid];
+    const unsigned f = sh.flat[tid];
+    int rank = 0;
+    for (int j = 0; j < entries; ++j) rank += before(sh.value[j], sh.flat[j], c, f);
+    if (c > -INFINITY && rank < a.select) put(rank, c, f);
   }
   // ---- fewer candidates than ranks: minus infinities in order.  (All finite
   // ones are taken then, less than `select`, so nearly every token is one.)

@@ -34,16 +34,22 @@ __device__ __forceinline__ int row_sequence(const PagedBatch &b, int row) {
 }
 
 // The searches for a row's or group's sequence meet only some sequences where
-// row starts do not ascend, and none without rows: with row starts, every
-// sequence's data are looked at here, spread over the launch.
-__device__ __forceinline__ void report_batch(const PagedBatch &b) {
-  if (!b.starts || blockIdx.y) return;
-  for (int s = blockIdx.x * kAppendThreads + threadIdx.x; s < b.sequences; s += gridDim.x * kAppendThreads) {
+// row starts do not ascend, and none without rows: with row starts, the last
+// workgroups of a launch look at every sequence's data, a thread each, and do
+// nothing else.  (In the others, it was 1 us of 41.)
+__host__ __device__ __forceinline__ int report_groups(const PagedBatch &b) {
+  return b.starts ? (b.sequences + kAppendThreads - 1) / kAppendThreads : 0;
+}
+__device__ __forceinline__ bool report_batch(const PagedBatch &b) {
+  const int group = int(blockIdx.x) - int(gridDim.x) + report_groups(b), s = group * kAppendThreads + threadIdx.x;
+  if (group < 0) return false;
+  if (blockIdx.y == 0 && s < b.sequences) {
     int first, end;
     dev::row_range(b, s, first, end);
     dev::own_length(b, s);
     dev::prefix_length(b, s / b.share);
   }
+  return true;
 }
 
 template <int E, typename T>
@@ -53,7 +59,7 @@ __global__ __launch_bounds__(kAppendThreads) void k_paged_append(const PagedCach
 #pragma clang fp contract(off)
   __shared__ double cs[kAppendMaxDim / 2], sn[kAppendMaxDim / 2];
   const int row = blockIdx.x, dim = c.dim, half = dim / 2, tid = threadIdx.x;
-  report_batch(b);
+  if (report_batch(b)) return;
   const int s = row_sequence(b, row);
   if (s < 0) return;
   int first, end;
@@ -128,13 +134,13 @@ __global__ __launch_bounds__(kAppendThreads) void k_paged_append_groups(const Pa
 #pragma clang fp contract(off)
   extern __shared__ double2 turn[];  // [32 tokens][dim / 2]
   const int id = blockIdx.x, dim = c.dim, half = dim / 2, tid = threadIdx.x;
-  report_batch(b);
+  if (report_batch(b)) return;
   int s = 0;
   for (int step = 1 << 16; step; step >>= 1)  // the last sequence whose first group is not behind this one
     if (s + step < b.sequences && first_group(b, s + step) <= id) s += step;
   int first, end;
-  dev::row_range(b, s, first, end);
-  const int length = dev::own_length(b, s), start = length - (end - first);  // own position of row `first`
+  dev::row_range<false>(b, s, first, end);
+  const int length = dev::own_length<false>(b, s), start = length - (end - first);  // own position of row `first`
   if (first == end) return;
   if (start < 0) {  // more rows than keys
     if (tid == 0) atomicOr(b.err, kPagedErr);
@@ -151,7 +157,7 @@ __global__ __launch_bounds__(kAppendThreads) void k_paged_append_groups(const Pa
       const double f = pow(double(theta), -2.0 * double(j) / double(dim));
       const int t0 = part * per;
       double sn, cn, ss, cs;
-      sincos(double(low + t0 + dev::prefix_length(b, s / b.share)) * f, &sn, &cn);
+      sincos(double(low + t0 + dev::prefix_length<false>(b, s / b.share)) * f, &sn, &cn);
       sincos(f, &ss, &cs);
       for (int t = t0; t < min(t0 + per, count); ++t) {
         turn[t * half + j] = {cn, sn};
@@ -356,7 +362,7 @@ void paged_append_launch(const PagedCache &c, const PagedBatch &b, const float *
   // and 8 heads, 128 channels: 53 us with workgroups per row, 41 in groups.
   if (b.starts && b.rows >= 2 * b.sequences) {
     const int groups = b.rows / kAppendGroup + 2 * b.sequences;
-    const dim3 grid(groups, std::max(1, std::min(16, 4096 / groups)));
+    const dim3 grid(groups + report_groups(b), std::max(1, std::min(16, 4096 / groups)));
     const size_t lds = size_t(kAppendGroup) * c.dim / 2 * sizeof(double2);
     if (c.bf16)
       k_paged_append_groups<8, __bf16><<<grid, kAppendThreads, lds, s>>>(c, b, k, v, q, q_out, heads, theta);
@@ -366,7 +372,7 @@ void paged_append_launch(const PagedCache &c, const PagedBatch &b, const float *
     return;
   }
   const int items = ((q ? heads : 0) + 3 * c.kv_heads) * c.dim / 2;
-  const dim3 grid(b.rows, std::min((items + kAppendThreads - 1) / kAppendThreads, b.rows < 64 ? 16 : 2));
+  const dim3 grid(b.rows + report_groups(b), std::min((items + kAppendThreads - 1) / kAppendThreads, b.rows < 64 ? 16 : 2));
   if (c.bf16)
     k_paged_append<8, __bf16><<<grid, kAppendThreads, 0, s>>>(c, b, k, v, q, q_out, heads, theta);
   else
