@@ -8,7 +8,11 @@
 // result, and only tiles whose best reaches T (`select` of them, but for ties)
 // are read again.  What reaches T there, a few times `select` candidates, is
 // ranked by counting.  The tile is chosen small enough that a group has several
-// times `select` of them, down to a wave's width.
+// times `select` of them, down to a wave's width.  Where more than 512 reach T
+// (ties: flat logits, or logits masked with a large finite value, all of which
+// round to one fp32 candidate), every wave keeps its best in order in one more
+// pass, and their lists are ranked: 8 groups of 8 beams over 151936 masked
+// tokens, 16 selected, 490 us (11.4 ms with a pass over all of them per rank).
 //
 // Candidates are compared in 64 bits.  Logits of one beam are exact there; two
 // beams' normalisers carry the roundings of fp32 sums, so the order across
@@ -32,7 +36,7 @@ namespace {
 
 constexpr int kScanThreads = 256, kMergeThreads = 1024;
 constexpr int kPerLaneMax = 16;
-constexpr int kList = 4096;  // tiles read again and candidates ranked, at most; more (ties) go by rounds
+constexpr int kList = 4096;  // tiles read again and candidates in LDS, at most; with more (ties) all tiles are looked at
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct TileStat {
@@ -207,6 +211,8 @@ __global__ __launch_bounds__(kMergeThreads) void k_beam_merge(const BeamArgs a, 
   auto reaches = [&](double c) { return c > -INFINITY && dev::order_bits(float(c)) >= limit; };
   if (count <= kList)
     for (int x = wave; x < count; x += kMergeThreads / 64) {
+      // (The list has run over: the tiles are read again below.)
+      if (__hip_atomic_load(&sh.found, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP) > kList) break;
       const int i = sh.list[x], b = i / tiles, t = i - b * tiles;
       if (sh.kind[b] == kDone) {
         if (lane == 0) {

@@ -98,6 +98,46 @@ def test_select_of_odd_values(ctx, rng):
     check_select(ctx, logits[[4, 3, 4]], scores[:3], np.array([1, 0, 0], np.int32), 1, 3, vocab, 64, 2)
 
 
+def test_select_of_finitely_masked_logits(ctx, rng):
+    """Constrained decoding masks with a large negative value: with fewer allowed tokens than ranks nearly every token
+    ties.  The selection is the defined one, and costs a further pass over the logits, not one per rank: more than a
+    hundred times an unmasked call (20 us) would be a pass per rank (11 ms)."""
+    groups, beams, vocab, k = 8, 8, 151936, 16
+    n = groups * beams
+    free_logits = (3 * rng.standard_normal((n, vocab))).astype(np.float32)
+    scores = (-5 * rng.random(n)).astype(np.float32)
+    forced, few, low = (np.full((n, vocab), m, np.float32) for m in (-1e9, -1e9, -3.4028235e38))
+    forced[np.arange(n), rng.integers(0, vocab, n)] = 1.5
+    few[:, 5000:5003] = rng.standard_normal((n, 3))
+    low[:, 77] = 0.25
+    took = {}
+    for name, x in (("free", free_logits), ("forced", forced), ("few", few), ("lowest", low), ("flat", np.zeros_like(low))):
+        check_select(ctx, x, scores, None, groups, beams, vocab, k)
+        tl, ts, found = up(ctx, x), up(ctx, scores), [ctx.NewTensor(groups * k) for _ in range(3)]
+        times = []
+        for _ in range(6):
+            ctx.EventRecord(0)
+            ctx.BeamSelect(*found, tl, ts, None, groups, beams, vocab, k)
+            ctx.EventRecord(1)
+            ctx.Flush()
+            times.append(ctx.EventElapsedMs(0, 1))
+        took[name] = min(times)
+        free(ctx, tl, ts, *found)
+    assert all(t <= 100 * took["free"] for t in took.values()), took
+
+
+def test_select_of_thousands_above_the_bound(ctx, rng):
+    """Lists of candidates too long to be ranked at once: distinct, in ascending order, and with ended beams among ties."""
+    for groups, beams, vocab, k in ((1, 64, 2000, 64), (2, 3, 1500, 64), (1, 2, 40000, 33)):
+        n = groups * beams
+        for logits in (rng.standard_normal((n, vocab)), np.broadcast_to(np.arange(vocab) / 64, (n, vocab)),
+                       rng.integers(0, 2, (n, vocab)), np.full((n, vocab), -1e9)):
+            scores = np.where(np.arange(n) % beams == beams - 1, np.float32(0), np.float32(-np.inf))
+            check_select(ctx, logits.astype(np.float32), scores, None, groups, beams, vocab, k)  # one live beam
+            done = (np.arange(n) % 2).astype(np.int32)
+            check_select(ctx, logits.astype(np.float32), np.full(n, -1.5, np.float32), done, groups, beams, vocab, k, 9)
+
+
 def test_select_refusals(ctx):
     n = 8 * 100
     logits, scores, done, p, t, s, small = (ctx.NewTensor(x) for x in (n, 8, 8, 16, 16, 16, 7))
