@@ -456,7 +456,9 @@ typedef struct {
  * and may have a prefix before their own keys, kept once: prefix_tables
  * [sequences / share][prefix_pages] and prefix_lengths [sequences / share],
  * both NULL without.  Row i of n of a sequence has own position
- * length - n + i, and absolute position prefix length + own position. */
+ * length - n + i, and absolute position prefix length + own position.
+ * A call's result is none of these tensors (but the lengths of
+ * qnn_paged_advance, which are no other one of them). */
 typedef struct {
   qnn_tensor *tables, *lengths, *starts, *prefix_tables, *prefix_lengths;
   int32_t sequences, rows, table_pages, prefix_pages, share;

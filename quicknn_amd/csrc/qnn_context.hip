@@ -2600,6 +2600,13 @@ PagedCache paged_cache(qnn_ctx_s *ctx, const qnn_paged_cache *c) {
   return p;
 }
 
+// What a call writes shall not be what its kernels read the batch from, more
+// than once in a call: their shares would disagree.
+void check_result(const qnn_paged_batch *b, const qnn_tensor *t) {
+  for (const qnn_tensor *x : {b->tables, b->lengths, b->starts, b->prefix_tables, b->prefix_lengths})
+    if (x && x == t) fail(QNN_E_ARGUMENT, "paged batch: a result is one of its tensors");
+}
+
 int paged_shift(int page_size) { return __builtin_ctz(unsigned(page_size)); }
 
 // A batch over pages of `page_size` tokens, `page_count` of them.
@@ -2659,8 +2666,10 @@ int qnn_paged_append(qnn_ctx *ctx, const qnn_paged_cache *cache, const qnn_paged
       check_tensor(ctx, q, int64_t(b.rows) * heads * c.dim);
       check_tensor(ctx, q_out, int64_t(b.rows) * heads * c.dim);
       if (q_out == k || q_out == v || q_out == cache->pages) fail(QNN_E_ARGUMENT, "paged append: q_out is an input");
+      check_result(batch, q_out);
     }
     if (k == cache->pages || v == cache->pages || q == cache->pages) fail(QNN_E_ARGUMENT, "paged append: rows in the cache");
+    check_result(batch, cache->pages);
     paged_append_launch(c, b, k->ptr, v->ptr, q ? q->ptr : nullptr, q ? q_out->ptr : nullptr, heads, theta, ctx->stream);
     return QNN_OK;
   });
@@ -2672,6 +2681,8 @@ int qnn_paged_advance(qnn_ctx *ctx, const qnn_paged_batch *batch, int page_size)
     if (page_size != 32 && page_size != 64 && page_size != 128 && page_size != 256)
       fail(QNN_E_NOT_SUPPORTED, "paged cache: pages of 32, 64, 128 or 256 tokens");
     const PagedBatch b = paged_batch(ctx, batch, page_size, 1);
+    for (const qnn_tensor *t : {batch->tables, batch->starts, batch->prefix_tables, batch->prefix_lengths})
+      if (t == batch->lengths) fail(QNN_E_ARGUMENT, "paged advance: the lengths are another tensor of the batch");
     paged_advance_launch(reinterpret_cast<int *>(batch->lengths->ptr), b, ctx->stream);
     return QNN_OK;
   });
@@ -2690,6 +2701,7 @@ int qnn_paged_attention(qnn_ctx *ctx, qnn_tensor *dst, qnn_tensor *q, const qnn_
     check_tensor(ctx, q, int64_t(a.b.rows) * heads * a.c.dim);
     check_tensor(ctx, dst, int64_t(a.b.rows) * heads * a.c.dim);
     if (dst == q || dst == cache->pages || q == cache->pages) fail(QNN_E_ARGUMENT, "paged attention: dst is an input");
+    check_result(batch, dst);
     a.q = q->ptr;
     a.out = dst->ptr;
     a.heads = heads;
@@ -2712,8 +2724,8 @@ int qnn_paged_reorder(qnn_ctx *ctx, const qnn_paged_batch *batch, qnn_tensor *ne
     if (b.share > 64) fail(QNN_E_NOT_SUPPORTED, "paged reorder: at most 64 sequences per group");
     check_tensor(ctx, parents, b.sequences);
     check_tensor(ctx, new_tables, int64_t(b.sequences) * b.table_pages);
-    if (new_tables == batch->tables || new_tables == parents || new_tables == batch->lengths)
-      fail(QNN_E_ARGUMENT, "paged reorder: the new tables are an input");
+    if (new_tables == parents) fail(QNN_E_ARGUMENT, "paged reorder: the new tables are an input");
+    check_result(batch, new_tables);
     std::vector<PagedCache> all(count);
     for (int i = 0; i < count; ++i) {
       all[i] = paged_cache(ctx, caches + i);
@@ -2722,8 +2734,8 @@ int qnn_paged_reorder(qnn_ctx *ctx, const qnn_paged_batch *batch, qnn_tensor *ne
         fail(QNN_E_ARGUMENT, "paged reorder: caches of different geometry");
       for (int j = 0; j < i; ++j)
         if (all[j].pages == all[i].pages) fail(QNN_E_ARGUMENT, "paged reorder: the same cache twice");
-      if (new_tables == caches[i].pages || parents == caches[i].pages || batch->tables == caches[i].pages)
-        fail(QNN_E_ARGUMENT, "paged reorder: tables in a cache");
+      if (new_tables == caches[i].pages || parents == caches[i].pages) fail(QNN_E_ARGUMENT, "paged reorder: tables in a cache");
+      check_result(batch, caches[i].pages);
     }
     for (int first = 0; first < count; first += kReorderLayers) {
       PagedLayers layers{};

@@ -111,3 +111,35 @@ assert rec.rec_allocations() == before + 1
 column = 4 * ({dim} + 4)
 assert rec.rec_largest() <= (2 * rows * {heads} + 2 * 512 * (32 + 128)) * column + (1 << 20), rec.rec_largest()
 """)
+
+
+def test_results_over_the_batchs_own_data_are_refused(host):
+    """Kernels read tables, lengths and starts many times in a call: a result over them would change them meanwhile."""
+    host("""
+B = hip.DT_BF16
+words = hip.PagedCache.words(B, 8, 64, 2, 64)
+big = dict(tables=8, lengths=4, starts=5, prefix_tables=4, prefix_lengths=2)
+t = {n: ctx.NewTensor(words) for n in big}
+cache = hip.PagedCache(ctx.NewTensor(words), B, 8, 64, 2, 64)
+q, k, v, out, parents = (ctx.NewTensor(4 * 4 * 64) for _ in range(5))
+
+def batch(**kw):
+    return hip.PagedBatch(**{**dict(t, sequences=4, rows=4, table_pages=2, prefix_pages=2, share=2), **kw})
+
+b = batch()
+ctx.PagedAttention(out, q, cache, b, 4)
+ctx.PagedAppend(cache, b, k, v, q, out, 4, 1e4)
+ctx.PagedAdvance(b, 64)
+ctx.PagedReorder(b, out, parents, [cache])
+A = hip.EArgumentException
+for name, x in t.items():
+    raises(A, ctx.PagedAttention, x, q, cache, b, 4)
+    raises(A, ctx.PagedAppend, cache, b, k, v, q, x, 4, 1e4)
+    raises(A, ctx.PagedReorder, b, x, parents, [cache])
+    if name != "lengths":
+        raises(A, ctx.PagedAdvance, batch(lengths=x), 64)
+    inside = hip.PagedCache(x, B, 8, 64, 2, 64)
+    raises(A, ctx.PagedAppend, inside, b, k, v, q, out, 4, 1e4)
+    raises(A, ctx.PagedReorder, b, out, parents, [cache, inside])
+ctx.Flush()
+""")
