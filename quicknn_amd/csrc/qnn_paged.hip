@@ -350,7 +350,8 @@ __global__ __launch_bounds__(256) void k_gather_rows(uint32_t *dst, const uint32
   const int r = blockIdx.x, from = indices[r];
   const bool ok = unsigned(from) < unsigned(src_rows);
   if (!ok && threadIdx.x == 0) atomicOr(err, kPagedErr);
-  for (int i = blockIdx.y * 256 + threadIdx.x; i < cols; i += gridDim.y * 256)
+  // (unsigned: a row may end less than a step below 2^31)
+  for (unsigned i = blockIdx.y * 256 + threadIdx.x; i < unsigned(cols); i += gridDim.y * 256)
     dst[size_t(r) * cols + i] = ok ? src[size_t(from) * cols + i] : 0u;
 }
 
@@ -395,7 +396,7 @@ void paged_reorder_launch(int *new_tables, const PagedBatch &b, const int *paren
 
 void gather_rows_launch(float *dst, const float *src, const int *indices, int rows, int cols, int src_rows, int *err,
                         hipStream_t s) {
-  const dim3 grid(rows, std::min((cols + 1023) / 1024, 64));
+  const dim3 grid(rows, std::min((cols - 1) / 1024 + 1, 64));
   k_gather_rows<<<grid, 256, 0, s>>>(reinterpret_cast<uint32_t *>(dst), reinterpret_cast<const uint32_t *>(src), indices,
                                      cols, src_rows, err);
   hip_check(hipGetLastError(), "gather rows launch");

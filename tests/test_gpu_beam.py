@@ -138,6 +138,31 @@ def test_select_of_thousands_above_the_bound(ctx, rng):
             check_select(ctx, logits.astype(np.float32), np.full(n, -1.5, np.float32), done, groups, beams, vocab, k, 9)
 
 
+def test_select_of_a_vocabulary_that_fills_a_tensor(ctx, rng):
+    """One beam of nearly 2^31 tokens: the last ones count, in the sum and among the selected."""
+    pattern, k = rng.standard_normal((5, 1000)).astype(np.float32), 6
+    rows = (2 ** 31 - 1) // 1000
+    vocab = rows * 1000
+    kinds = (np.arange(rows) % 5).astype(np.int32)
+    t, i, logits = up(ctx, pattern), words(ctx, kinds), ctx.NewTensor(vocab)
+    ctx.GatherRows(logits, t, i, rows, 1000)
+    places = [vocab - 1, 3, vocab - 700, vocab - 1100, vocab // 2, 1 << 30]
+    values = [9.0, 9.0, 8.5, 8.0, 7.5, 7.0]
+    total = np.bincount(kinds) @ np.exp(pattern.astype(np.float64)).sum(1)
+    for p, v in zip(places, values):
+        one = up(ctx, np.array([v], np.float32))
+        ctx.Copy(logits, one, 1, p)
+        ctx.Recycle(one)
+        total += np.exp(v) - np.exp(np.float64(pattern[kinds[p // 1000], p % 1000]))
+    scores, found = up(ctx, np.array([-1.5], np.float32)), [ctx.NewTensor(k) for _ in range(3)]
+    ctx.BeamSelect(*found, logits, scores, None, 1, 1, vocab, k)
+    assert ctx.Download(found[0], dtype=np.int32).tolist() == [0] * k
+    assert ctx.Download(found[1], dtype=np.int32).tolist() == [places[j] for j in (1, 0, 2, 3, 4, 5)]
+    want = -1.5 + np.array(values) - np.log(total)
+    assert np.all(np.abs(ctx.Download(found[2]) - want) <= 2e-6 + 2.0 ** -23 * np.abs(want))
+    free(ctx, t, i, logits, scores, *found)
+
+
 def test_select_refusals(ctx):
     n = 8 * 100
     logits, scores, done, p, t, s, small = (ctx.NewTensor(x) for x in (n, 8, 8, 16, 16, 16, 7))

@@ -484,6 +484,27 @@ def test_gather_rows(ctx, rng, rows, cols, src_rows):
     free(ctx, t, i, dst)
 
 
+def test_gather_of_a_row_that_fills_a_tensor(ctx, rng):
+    """One row of nearly 2^31 words, the most that a tensor holds: copied to its end, and nothing behind it."""
+    pattern = rng.integers(0, 1 << 31, (7, 1000), dtype=np.int32)
+    rows = (2 ** 31 - 1) // 1000
+    kinds = (np.arange(rows) * 5 // 3 % 7).astype(np.int32)
+    t, i, src, dst = words(ctx, pattern), words(ctx, kinds), ctx.NewTensor(2 ** 31 - 1), ctx.NewTensor(2 ** 31 - 1)
+    ctx.GatherRows(src, t, i, rows, 1000)  # 2147483 rows
+    zero, tail = words(ctx, np.zeros(647, np.int32)), ctx.NewTensor(647)
+    ctx.Copy(dst, zero, 647, rows * 1000)
+    only = words(ctx, [0])
+    for width in ((rows - 1) * 1000, rows * 1000):  # less than a step of the loop, and of a workgroup, below 2^31
+        ctx.GatherRows(dst, src, only, 1, width, 1)
+    look = np.array([0, 1, 16383, rows // 2, rows - 17, rows - 2, rows - 1], np.int32)
+    at, out = words(ctx, look), ctx.NewTensor(look.size * 1000)
+    ctx.GatherRows(out, dst, at, look.size, 1000)
+    assert np.array_equal(ctx.Download(out, dtype=np.int32).reshape(-1, 1000), pattern[kinds[look]])
+    ctx.Copy(tail, dst, 647, 0, rows * 1000)
+    assert not np.any(ctx.Download(tail, dtype=np.int32))
+    free(ctx, t, i, src, dst, zero, tail, only, at, out)
+
+
 # ---------------------------------------------------------------- reorder
 def reorder_plan(tables, length, parents, share, page):
     """New tables and (from page, to page) copies, by the documented rule."""
