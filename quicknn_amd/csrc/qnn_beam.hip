@@ -201,10 +201,10 @@ __global__ __launch_bounds__(kMergeThreads) void k_beam_merge(const BeamArgs a, 
     count = sh.kept;
   }
   const unsigned limit = bound;
-  const int span = 64 * per_lane;
-  // Lane `lane` of the wave that calls it with token v of beam b.
+  // (Unsigned from here: the last tile may end behind 2^31.)
+  const unsigned span = 64 * per_lane, vocab = a.vocab;
+  // The candidate of token v of beam b.
   auto value_of = [&](int b, int v) -> double {
-    if (v >= a.vocab) return -INFINITY;
     if (sh.kind[b] == kLive) return candidate(b, a.logits[size_t(first + b) * a.vocab + v]);
     return sh.kind[b] == kDone && v == a.end ? sh.score[b] : -INFINITY;
   };
@@ -217,7 +217,7 @@ __global__ __launch_bounds__(kMergeThreads) void k_beam_merge(const BeamArgs a, 
       if (sh.kind[b] == kDone) {
         if (lane == 0) {
           const int at = atomicAdd(&sh.found, 1);
-          if (at < kList) sh.value[at] = sh.score[b], sh.flat[at] = unsigned(b) * a.vocab + a.end;
+          if (at < kList) sh.value[at] = sh.score[b], sh.flat[at] = b * vocab + a.end;
         }
         continue;
       }
@@ -225,14 +225,14 @@ __global__ __launch_bounds__(kMergeThreads) void k_beam_merge(const BeamArgs a, 
       const float *row = a.logits + size_t(first + b) * a.vocab;
       float y[kPerLaneMax];
 #pragma unroll
-      for (int j = 0; j < kPerLaneMax; ++j) y[j] = row[min(t * span + min(j, per_lane - 1) * 64 + lane, a.vocab - 1)];
+      for (int j = 0; j < kPerLaneMax; ++j) y[j] = row[min(t * span + min(j, per_lane - 1) * 64 + lane, vocab - 1)];
 #pragma unroll
       for (int j = 0; j < kPerLaneMax; ++j) {
-        const int v = t * span + j * 64 + lane;
-        const double c = j < per_lane && v < a.vocab ? candidate(b, y[j]) : -INFINITY;
+        const unsigned v = t * span + j * 64 + lane;
+        const double c = j < per_lane && v < vocab ? candidate(b, y[j]) : -INFINITY;
         if (reaches(c)) {
           const int at = atomicAdd(&sh.found, 1);
-          if (at < kList) sh.value[at] = c, sh.flat[at] = unsigned(b) * a.vocab + v;
+          if (at < kList) sh.value[at] = c, sh.flat[at] = b * vocab + v;
         }
       }
     }
@@ -240,8 +240,8 @@ __global__ __launch_bounds__(kMergeThreads) void k_beam_merge(const BeamArgs a, 
   const int found = count <= kList ? sh.found : kList + 1;
   auto put = [&](int rank, double c, unsigned flat) {
     const size_t at = size_t(group) * a.select + rank;
-    a.parents[at] = first + int(flat / unsigned(a.vocab));
-    a.tokens[at] = int(flat % unsigned(a.vocab));
+    a.parents[at] = first + int(flat / vocab);
+    a.tokens[at] = int(flat % vocab);
     a.best[at] = float(c);
   };
   int ranked = min(found, a.select), entries = found;
@@ -269,19 +269,19 @@ __global__ __launch_bounds__(kMergeThreads) void k_beam_merge(const BeamArgs a, 
     auto offer_tile = [&](int i) {
       const int b = i / tiles, t = i - b * tiles;
       if (sh.kind[b] == kDone) {
-        offer(lane == 0 ? sh.score[b] : -INFINITY, unsigned(b) * a.vocab + a.end);
+        offer(lane == 0 ? sh.score[b] : -INFINITY, b * vocab + a.end);
         return;
       }
       const float *row = a.logits + size_t(first + b) * a.vocab;
       for (int j0 = 0; j0 < per_lane; j0 += 8) {
         float y[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = row[min(t * span + min(j0 + j, per_lane - 1) * 64 + lane, a.vocab - 1)];
+        for (int j = 0; j < 8; ++j) y[j] = row[min(t * span + min(j0 + j, per_lane - 1) * 64 + lane, vocab - 1)];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const int v = t * span + (j0 + j) * 64 + lane;
-          const double c1 = j0 + j < per_lane && v < a.vocab ? candidate(b, y[j]) : -INFINITY;
-          offer(reaches(c1) ? c1 : -INFINITY, unsigned(b) * a.vocab + v);
+          const unsigned v = t * span + (j0 + j) * 64 + lane;
+          const double c1 = j0 + j < per_lane && v < vocab ? candidate(b, y[j]) : -INFINITY;
+          offer(reaches(c1) ? c1 : -INFINITY, b * vocab + v);
         }
       }
     };
@@ -313,10 +313,10 @@ __global__ __launch_bounds__(kMergeThreads) void k_beam_merge(const BeamArgs a, 
   // ---- fewer candidates than ranks: minus infinities in order.  (All finite
   // ones are taken then, less than `select`, so nearly every token is one.)
   if (ranked < a.select && wave == 0) {
-    const unsigned all = unsigned(a.beams) * unsigned(a.vocab);
+    const unsigned all = a.beams * vocab;
     for (unsigned f0 = 0; ranked < a.select && f0 < all; f0 += 64) {
       const unsigned f = f0 + lane;
-      const bool in = f < all && value_of(int(f / unsigned(a.vocab)), int(f % unsigned(a.vocab))) == -INFINITY;
+      const bool in = f < all && value_of(int(f / vocab), int(f % vocab)) == -INFINITY;
       const uint64_t mask = __ballot(in);
       const int rank = ranked + __popcll(mask & ((uint64_t(1) << lane) - 1));
       if (in && rank < a.select) put(rank, -INFINITY, f);
@@ -331,7 +331,7 @@ int per_lane_of(const BeamArgs &a) {
   while (e > 1 && int64_t(a.beams) * a.vocab / (64 * e) < 8 * a.select) e /= 2;
   return e;
 }
-int tiles_of(const BeamArgs &a) { return (a.vocab + 64 * per_lane_of(a) - 1) / (64 * per_lane_of(a)); }
+int tiles_of(const BeamArgs &a) { return (a.vocab - 1) / (64 * per_lane_of(a)) + 1; }
 
 }  // namespace
 

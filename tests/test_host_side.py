@@ -143,3 +143,14 @@ for name, x in t.items():
     raises(A, ctx.PagedReorder, b, out, parents, [cache, inside])
 ctx.Flush()
 """)
+
+
+def test_selection_of_the_largest_vocabulary(host):
+    """The workspace of a vocabulary within a tile of 2^31 tokens: 8 bytes per 1024."""
+    host("""
+vocab = 2 ** 31 - 1
+logits, scores, found = ctx.NewTensor(vocab), ctx.NewTensor(1), [ctx.NewTensor(4) for _ in range(3)]
+rec.rec_forget_largest()
+ctx.BeamSelect(*found, logits, scores, None, 1, 1, vocab, 4)
+assert rec.rec_largest() == 2 ** 21 * 8, rec.rec_largest()
+""")
