@@ -345,14 +345,16 @@ __global__ __launch_bounds__(kReorderThreads) void k_paged_reorder(int *new_tabl
 }
 
 // Rows of 32-bit words by index; an index outside gives zeros and the error word.
-__global__ __launch_bounds__(256) void k_gather_rows(uint32_t *dst, const uint32_t *src, const int *indices, int cols,
-                                                     int src_rows, int *err) {
-  const int r = blockIdx.x, from = indices[r];
-  const bool ok = unsigned(from) < unsigned(src_rows);
-  if (!ok && threadIdx.x == 0) atomicOr(err, kPagedErr);
-  // (unsigned: a row may end less than a step below 2^31)
-  for (unsigned i = blockIdx.y * 256 + threadIdx.x; i < unsigned(cols); i += gridDim.y * 256)
-    dst[size_t(r) * cols + i] = ok ? src[size_t(from) * cols + i] : 0u;
+__global__ __launch_bounds__(256) void k_gather_rows(uint32_t *dst, const uint32_t *src, const int *indices, int rows,
+                                                     int cols, int src_rows, int *err) {
+  for (unsigned r = blockIdx.x; r < unsigned(rows); r += gridDim.x) {
+    const int from = indices[r];
+    const bool ok = unsigned(from) < unsigned(src_rows);
+    if (!ok && threadIdx.x == 0) atomicOr(err, kPagedErr);
+    // (unsigned: a row may end less than a step below 2^31)
+    for (unsigned i = blockIdx.y * 256 + threadIdx.x; i < unsigned(cols); i += gridDim.y * 256)
+      dst[size_t(r) * cols + i] = ok ? src[size_t(from) * cols + i] : 0u;
+  }
 }
 
 }  // namespace
@@ -396,9 +398,10 @@ void paged_reorder_launch(int *new_tables, const PagedBatch &b, const int *paren
 
 void gather_rows_launch(float *dst, const float *src, const int *indices, int rows, int cols, int src_rows, int *err,
                         hipStream_t s) {
-  const dim3 grid(rows, std::min((cols - 1) / 1024 + 1, 64));
+  // (A launch counts its threads along x in 32 bits.)
+  const dim3 grid(std::min(rows, 1 << 22), std::min((cols - 1) / 1024 + 1, 64));
   k_gather_rows<<<grid, 256, 0, s>>>(reinterpret_cast<uint32_t *>(dst), reinterpret_cast<const uint32_t *>(src), indices,
-                                     cols, src_rows, err);
+                                     rows, cols, src_rows, err);
   hip_check(hipGetLastError(), "gather rows launch");
 }
 

@@ -15,7 +15,7 @@ namespace {
 struct Dim3 {
   uint32_t x, y, z;
 };
-constexpr int kOutOfMemory = 2;
+constexpr int kOutOfMemory = 2, kInvalidConfiguration = 9;
 int last_error = 0;
 std::map<void *, size_t> live;
 std::map<const void *, std::string> names;
@@ -50,7 +50,9 @@ int hipGetLastError() {
   last_error = 0;
   return e;
 }
-const char *hipGetErrorString(int e) { return e == kOutOfMemory ? "out of memory" : "no error"; }
+const char *hipGetErrorString(int e) { 
+  return e == kOutOfMemory ? "out of memory" : e == kInvalidConfiguration ? "invalid configuration" : "no error";
+}
 int hipGetDeviceCount(int *n) { return *n = 1, 0; }
 int hipSetDevice(int) { return 0; }
 int hipDeviceGetAttribute(int *v, int, int) { return *v = 256, 0; }
@@ -95,7 +97,10 @@ int hipEventElapsedTime(float *ms, void *, void *) { return *ms = 0, 0; }
 int hipFuncSetAttribute(const void *, int, int) { return 0; }
 int hipOccupancyMaxActiveBlocksPerMultiprocessor(int *n, const void *, int, size_t) { return *n = 1, 0; }
 int hipGetSymbolAddress(void **p, const void *) { return (*p = map_bytes(size_t(64) << 20)) ? 0 : kOutOfMemory; }
-int hipLaunchKernel(const void *f, Dim3, Dim3, void **, size_t, void *) {
+int hipLaunchKernel(const void *f, Dim3 grid, Dim3 block, void **, size_t, void *) {
+  // Threads along a dimension are counted in 32 bits; y and z take 65535 workgroups.
+  if (!grid.x || !grid.y || !grid.z || uint64_t(grid.x) * block.x > 0xffffffffull || grid.y > 65535 || grid.z > 65535)
+    return last_error = kInvalidConfiguration;
   launched += names[f] + "\n";
   return 0;
 }

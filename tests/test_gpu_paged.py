@@ -484,6 +484,15 @@ def test_gather_rows(ctx, rng, rows, cols, src_rows):
     free(ctx, t, i, dst)
 
 
+def test_gather_of_more_rows_than_workgroups(ctx, rng):
+    rows = (1 << 24) + 5
+    src, idx = rng.integers(0, 1 << 31, 1000, dtype=np.int32), rng.integers(0, 1000, rows, dtype=np.int32)
+    t, i, dst = words(ctx, src), words(ctx, idx), ctx.NewTensor(rows)
+    ctx.GatherRows(dst, t, i, rows, 1)
+    assert np.array_equal(ctx.Download(dst, dtype=np.int32), src[idx])
+    free(ctx, t, i, dst)
+
+
 def test_gather_of_a_row_that_fills_a_tensor(ctx, rng):
     """One row of nearly 2^31 words, the most that a tensor holds: copied to its end, and nothing behind it."""
     pattern = rng.integers(0, 1 << 31, (7, 1000), dtype=np.int32)

@@ -154,3 +154,14 @@ rec.rec_forget_largest()
 ctx.BeamSelect(*found, logits, scores, None, 1, 1, vocab, 4)
 assert rec.rec_largest() == 2 ** 21 * 8, rec.rec_largest()
 """)
+
+
+@pytest.mark.parametrize("rows,cols", [(1 << 24, 1), (2 ** 31 - 1, 1), (20_000_003, 100), (1, 2 ** 31 - 1)])
+def test_gather_of_many_rows(host, rows, cols):
+    """As many rows as tensors hold, in one launch."""
+    host(f"""
+dst, src, indices = ctx.NewTensor({rows * cols}), ctx.NewTensor({cols}), ctx.NewTensor({rows})
+ctx.GatherRows(dst, src, indices, {rows}, {cols})
+ctx.Flush()
+assert rec.rec_launched().count(b"k_gather_rows") == 1
+""")
