@@ -493,7 +493,9 @@ int qnn_paged_attention(qnn_ctx *ctx, qnn_tensor *dst, qnn_tensor *q, const qnn_
  * from then on.  The page that is partly filled is taken over by a parent's
  * first child; further children, in order, get the pages of parents without
  * children, in order, with a copy of the 32-token blocks in use, in each of the
- * `count` caches (the layers, of one geometry, all addressed by these tables). */
+ * `count` caches (the layers, of one geometry, all addressed by these tables).
+ * A page that is partly filled belongs to one sequence when the call is made.
+ * QNN_E_RANGE when a group's tables hold more than 2^30 page ids. */
 int qnn_paged_reorder(qnn_ctx *ctx, const qnn_paged_batch *batch, qnn_tensor *new_tables, qnn_tensor *parents,
                       const qnn_paged_cache *caches, int count);
 /* dst[r] = src[indices[r]]: rows of `cols` words; zeros for an index outside src_rows. */

@@ -2722,6 +2722,8 @@ int qnn_paged_reorder(qnn_ctx *ctx, const qnn_paged_batch *batch, qnn_tensor *ne
     const PagedCache shape = paged_cache(ctx, caches);
     const PagedBatch b = paged_batch(ctx, batch, shape.page_size, shape.page_count);
     if (b.share > 64) fail(QNN_E_NOT_SUPPORTED, "paged reorder: at most 64 sequences per group");
+    if (int64_t(b.share) * b.table_pages > (1 << 30))  // counted in 32 bits, in steps of a workgroup
+      fail(QNN_E_RANGE, "paged reorder: more than 2^30 page ids in a group's tables");
     check_tensor(ctx, parents, b.sequences);
     check_tensor(ctx, new_tables, int64_t(b.sequences) * b.table_pages);
     if (new_tables == parents) fail(QNN_E_ARGUMENT, "paged reorder: the new tables are an input");

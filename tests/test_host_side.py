@@ -165,3 +165,15 @@ ctx.GatherRows(dst, src, indices, {rows}, {cols})
 ctx.Flush()
 assert rec.rec_launched().count(b"k_gather_rows") == 1
 """)
+
+
+def test_reorder_of_tables_past_32_bits_is_refused(host):
+    """64 sequences with 2^25 - 1 pages each: the copy of their tables steps past 2^31."""
+    host("""
+pages = 2 ** 25 - 1
+cache = hip.PagedCache(ctx.NewTensor(hip.PagedCache.words(hip.DT_BF16, 1, 32, 1, 16)), hip.DT_BF16, 1, 32, 1, 16)
+tables, new, lengths, parents = (ctx.NewTensor(n) for n in (64 * pages, 64 * pages, 64, 64))
+raises(hip.ERangeError, ctx.PagedReorder, hip.PagedBatch(tables, lengths, 64, 64, pages, share=64), new, parents, [cache])
+ctx.PagedReorder(hip.PagedBatch(tables, lengths, 64, 64, 2 ** 24, share=64), new, parents, [cache])
+ctx.Flush()
+""")
