@@ -408,13 +408,32 @@ def _th(t: Tensor | None):
     return None if t is None else t.handle
 
 
-class PagedCache:
+class _Described:
+    """Attributes that are the fields of a C descriptor, ``_c``, which follows them when they are set."""
+
+    _struct: type
+
+    def __init__(self, **fields):
+        self._c = self._struct()
+        for name, value in fields.items():
+            setattr(self, name, value)
+
+    def __setattr__(self, name, value):
+        kind = dict(self._struct._fields_).get(name)
+        if kind is None and name != "_c":
+            raise AttributeError(f"{type(self).__name__} has no field {name}")
+        if kind is not None:
+            setattr(self._c, name, _th(value) if kind is _vp else value)
+        object.__setattr__(self, name, value)
+
+
+class PagedCache(_Described):
     """qnn_paged_cache: the KV cache of one layer, in pages of ``page_size`` tokens kept in one tensor."""
 
+    _struct = _PagedCache
+
     def __init__(self, pages: Tensor, dtype: int, page_count: int, page_size: int, kv_heads: int, dim: int):
-        self.pages, self.dtype, self.page_count, self.page_size = pages, dtype, page_count, page_size
-        self.kv_heads, self.dim = kv_heads, dim
-        self._c = _PagedCache(_th(pages), dtype, page_count, page_size, kv_heads, dim)
+        super().__init__(pages=pages, dtype=dtype, page_count=page_count, page_size=page_size, kv_heads=kv_heads, dim=dim)
 
     @staticmethod
     def words(dtype: int, page_count: int, page_size: int, kv_heads: int, dim: int) -> int:
@@ -422,18 +441,17 @@ class PagedCache:
         return 2 * page_count * kv_heads * page_size * dim // (2 if dtype == DT_BF16 else 1)
 
 
-class PagedBatch:
+class PagedBatch(_Described):
     """qnn_paged_batch: sequences, their rows in a call and their page tables (words in tensors)."""
+
+    _struct = _PagedBatch
 
     def __init__(self, tables: Tensor, lengths: Tensor, sequences: int, rows: int, table_pages: int,
                  starts: Tensor | None = None, prefix_tables: Tensor | None = None,
                  prefix_lengths: Tensor | None = None, prefix_pages: int = 0, share: int = 1):
-        self.tables, self.lengths, self.starts = tables, lengths, starts
-        self.prefix_tables, self.prefix_lengths = prefix_tables, prefix_lengths
-        self.sequences, self.rows, self.table_pages, self.prefix_pages, self.share = (sequences, rows, table_pages,
-                                                                                      prefix_pages, share)
-        self._c = _PagedBatch(_th(tables), _th(lengths), _th(starts), _th(prefix_tables), _th(prefix_lengths),
-                              sequences, rows, table_pages, prefix_pages, share)
+        super().__init__(tables=tables, lengths=lengths, starts=starts, prefix_tables=prefix_tables,
+                         prefix_lengths=prefix_lengths, sequences=sequences, rows=rows, table_pages=table_pages,
+                         prefix_pages=prefix_pages, share=share)
 
 
 # Contexts still open when the interpreter exits are destroyed by an atexit

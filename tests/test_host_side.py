@@ -177,3 +177,26 @@ raises(hip.ERangeError, ctx.PagedReorder, hip.PagedBatch(tables, lengths, 64, 64
 ctx.PagedReorder(hip.PagedBatch(tables, lengths, 64, 64, 2 ** 24, share=64), new, parents, [cache])
 ctx.Flush()
 """)
+
+
+def test_descriptors_follow_their_attributes(host):
+    """What is set on a cache's or batch's description after its making is what the next call takes."""
+    host("""
+a, b, q, out = (ctx.NewTensor(n) for n in (8 * 64 * 64, 8, 4 * 64, 4 * 64))
+cache = hip.PagedCache(a, hip.DT_F32, 4, 64, 1, 64)
+batch = hip.PagedBatch(b, b, 4, 4, 1)
+ctx.PagedAttention(out, q, cache, batch, 1)
+batch.rows = 3
+raises(hip.EArgumentException, ctx.PagedAttention, out, q, cache, batch, 1)
+batch.starts = b
+ctx.PagedAttention(out, q, cache, batch, 1)
+batch.starts, batch.rows, batch.tables = None, 4, None
+raises(hip.EArgumentException, ctx.PagedAttention, out, q, cache, batch, 1)
+batch.tables = b
+ctx.PagedAttention(out, q, cache, batch, 1)
+cache.page_count = 5
+raises(hip.EArgumentException, ctx.PagedAttention, out, q, cache, batch, 1)
+raises(AttributeError, setattr, batch, "length", b)
+assert (batch.rows, batch.tables, cache.page_count) == (4, b, 5)
+ctx.Flush()
+""")
