@@ -426,6 +426,9 @@ class _Described:
             setattr(self._c, name, _th(value) if kind is _vp else value)
         object.__setattr__(self, name, value)
 
+    def __copy__(self):  # with a descriptor of its own
+        return type(self)(**{name: getattr(self, name) for name, _ in self._struct._fields_})
+
 
 class PagedCache(_Described):
     """qnn_paged_cache: the KV cache of one layer, in pages of ``page_size`` tokens kept in one tensor."""

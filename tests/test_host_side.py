@@ -198,5 +198,10 @@ cache.page_count = 5
 raises(hip.EArgumentException, ctx.PagedAttention, out, q, cache, batch, 1)
 raises(AttributeError, setattr, batch, "length", b)
 assert (batch.rows, batch.tables, cache.page_count) == (4, b, 5)
+import copy
+other = copy.copy(cache)
+other.page_count = 4
+assert cache._c.page_count == 5
+ctx.PagedAttention(out, q, other, batch, 1)
 ctx.Flush()
 """)
