@@ -880,24 +880,138 @@ __global__ __launch_bounds__(256) void k_attn_merge_general(float *out, const fl
 // added in rank order, are one chain of k additions with a candidate per lane.
 // 151936 tokens, k = 40: 15 us (a bitonic sort per wave, a second one of the
 // four waves' lists, and the draw in one thread: 30).
-using dev::from_order_bits;
-using dev::group_topk;
-using dev::kSamplePerThread;
-using dev::kSampleThreads;
-using dev::kSampleTile;
-using dev::order_bits;
-using dev::rank_key;
-using dev::SampleShared;
+constexpr int kSampleThreads = 256;
+constexpr int kSamplePerThread = 16;
+constexpr int kSampleTile = kSampleThreads * kSamplePerThread;
 constexpr unsigned kNoToken = 0xffffffffu;
 constexpr float kLowest = -3.402823466e38f;
 
+using dev::order_bits;
+__device__ __forceinline__ float from_order_bits(uint32_t o) {
+  return __uint_as_float((o & 0x80000000u) ? (o & 0x7fffffffu) : ~o);
+}
+__device__ __forceinline__ uint64_t rank_key(float s, unsigned id) {
+  return isnan(s) ? 0ull : (uint64_t(order_bits(s)) << 32) | uint32_t(~id);
+}
 // The key of the reference's starting best (-FLT_MAX, 0xffffffff).
 __device__ __forceinline__ uint64_t floor_key() { return uint64_t(order_bits(kLowest)) << 32; }
+
+using dev::wave_max_u32;
+// Wave-wide maximum of 64-bit keys: the high words first; the low words only
+// among the lanes that hold the highest high word.
+__device__ __forceinline__ uint64_t wave_max_key(uint64_t v) {
+  const uint32_t hi = uint32_t(v >> 32), lo = uint32_t(v);
+  const uint32_t mh = wave_max_u32(hi);
+  const uint64_t at = __ballot(hi == mh);
+  uint32_t ml;
+  if (__popcll(at) == 1)
+    ml = uint32_t(__builtin_amdgcn_readlane(int(lo), __ffsll(static_cast<long long>(at)) - 1));
+  else
+    ml = wave_max_u32(hi == mh ? lo : 0u);
+  return (uint64_t(mh) << 32) | ml;
+}
+
+// k rounds over J candidate keys per lane: each takes the wave-wide best key
+// below the previous pick; keys at or below the floor are never picked.
+template <int J>
+__device__ __forceinline__ void rank_rounds(const uint64_t (&c)[J], int k, uint64_t *out) {
+  const uint64_t floor = floor_key();
+  uint64_t prev = ~0ull;
+  for (int rank = 0; rank < k; ++rank) {
+    uint64_t b = 0ull;
+#pragma unroll
+    for (int i = 0; i < J; ++i) {
+      const uint64_t v = c[i] < prev ? c[i] : 0ull;
+      b = v > b ? v : b;
+    }
+    uint64_t best = wave_max_key(b);
+    if (best < floor) best = floor;
+    if ((threadIdx.x & 63) == 0) out[rank] = best;
+    prev = best;
+  }
+}
 
 struct SampleArgs {
   int count, k, tiles, level0, merge;
   float temperature, top_p, penalty, uniform;
 };
+
+// Keys that are ranked by counting; more (ties, flat logits) are first cut to
+// each wave's own top-k by k rounds of the wave-wide maximum.  Counting costs
+// count x ceil(count / 256) LDS reads: 512 are about as long as 64 rounds.
+constexpr int kSampleCap = 512;
+struct SampleShared {
+  uint64_t cand[kSampleCap];
+  uint32_t t[4];
+  int count;
+};
+
+// The workgroup's ranked top-k (k <= 64) of its 4096 keys (16 per lane):
+// put(rank, key) for every rank below k, from one thread each.
+template <typename Put>
+__device__ __forceinline__ void group_topk(const uint64_t (&key)[kSamplePerThread], int k, SampleShared &sh, Put put) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const uint64_t floor = floor_key();
+  // The largest t with at least k half-lane maxima whose score bits reach it
+  // (0: fewer than k): every key of the wave's top-k reaches t, and every key
+  // of the workgroup's top-k reaches each wave's t.
+  uint32_t hm0 = 0, hm1 = 0;
+#pragma unroll
+  for (int i = 0; i < kSamplePerThread; ++i) {
+    const uint32_t h = uint32_t(key[i] >> 32);
+    if (i < kSamplePerThread / 2) hm0 = max(hm0, h);
+    else hm1 = max(hm1, h);
+  }
+  uint32_t t = 0;
+#pragma unroll 1
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t c = t | (1u << bit);
+    if (__popcll(__ballot(hm0 >= c)) + __popcll(__ballot(hm1 >= c)) >= k) t = c;
+  }
+  if (lane == 0) sh.t[wave] = t;
+  if (tid == 0) sh.count = 0;
+  __syncthreads();
+  t = max(max(sh.t[0], sh.t[1]), max(sh.t[2], sh.t[3]));
+  uint32_t keep = 0;
+  int mine = 0;
+#pragma unroll
+  for (int i = 0; i < kSamplePerThread; ++i) {
+    const bool in = key[i] > floor && uint32_t(key[i] >> 32) >= t;
+    keep |= uint32_t(in) << i;
+    mine += __popcll(__ballot(in));
+  }
+  int base = 0;
+  if (lane == 0) base = atomicAdd(&sh.count, mine);
+  base = __builtin_amdgcn_readfirstlane(base);
+  if (base + mine <= kSampleCap) {
+#pragma unroll
+    for (int i = 0; i < kSamplePerThread; ++i) {
+      const bool in = (keep >> i) & 1u;
+      const uint64_t mask = __ballot(in);
+      if (in) sh.cand[base + __popcll(mask & ((1ull << lane) - 1ull))] = key[i];
+      base += __popcll(mask);
+    }
+  }
+  __syncthreads();
+  int count = sh.count, above = count;
+  if (count > kSampleCap) {  // the same in every thread
+    __syncthreads();
+    rank_rounds<kSamplePerThread>(key, k, sh.cand + wave * k);
+    count = 4 * k;
+    __syncthreads();
+    above = 0;  // the lists end in floors
+    for (int j = 0; j < count; ++j) above += sh.cand[j] > floor;
+  }
+  for (int c = tid; c < count; c += kSampleThreads) {
+    const uint64_t v = sh.cand[c];
+    int rank = 0;
+#pragma unroll 8
+    for (int j = 0; j < count; ++j) rank += sh.cand[j] > v;
+    if (rank < k && v > floor) put(rank, v);  // keys above the floor are distinct
+  }
+  if (tid < k && tid >= above) put(tid, floor);  // ranks that no key took
+  __syncthreads();
+}
 
 __global__ __launch_bounds__(kSampleThreads) void k_sample(unsigned *dst, const float *logits, const unsigned *seen,
                                                            const uint64_t *in_keys, uint64_t *out_keys,
@@ -936,7 +1050,7 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample(unsigned *dst, const 
       if (item0 + unsigned(i) * 64 > end) key[i] = 0ull;
   }
   uint64_t *mine = out_keys + size_t(tile) * a.k;
-  group_topk(key, a.k, sh, floor_key(), [&](int rank, uint64_t v) {
+  group_topk(key, a.k, sh, [&](int rank, uint64_t v) {
     __hip_atomic_store(&mine[rank], v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   });
   if (!a.merge) return;
@@ -957,7 +1071,7 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample(unsigned *dst, const 
 #pragma unroll
   for (int i = 0; i < kSamplePerThread; ++i)
     if (wave * 1024 + i * 64 + lane >= count) key[i] = 0ull;
-  group_topk(key, a.k, sh, floor_key(), [&](int rank, uint64_t v) { top[rank] = v; });
+  group_topk(key, a.k, sh, [&](int rank, uint64_t v) { top[rank] = v; });
   if (wave == 0) {
 #pragma clang fp contract(off)
     const uint64_t v = lane < a.k ? top[lane] : 0ull;

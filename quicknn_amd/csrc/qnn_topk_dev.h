@@ -1,9 +1,6 @@
-// qnn_topk_dev.h -- the exact ranked top-k of a workgroup's keys, shared by
-// token sampling (qnn_decode.hip) and beam selection (qnn_beam.hip).
-//
-// A key holds the order-preserving bits of a score (-0 as +0) above the
-// inverted id, so a larger key is a higher score or, on equal scores, a lower
-// id; key 0 is none (NaN).
+// qnn_topk_dev.h -- what token sampling (qnn_decode.hip), beam selection
+// (qnn_beam.hip) and paged attention share: the bits of a score whose order as
+// unsigned words is the scores' order, and a wave's largest word.
 #pragma once
 #include <hip/hip_runtime.h>
 
@@ -12,19 +9,10 @@
 namespace qnn {
 namespace dev {
 
-constexpr int kSampleThreads = 256;
-constexpr int kSamplePerThread = 16;
-constexpr int kSampleTile = kSampleThreads * kSamplePerThread;
-
+// (-0 as +0.)
 __device__ __forceinline__ uint32_t order_bits(float s) {
   const uint32_t u = __float_as_uint(s == 0.0f ? 0.0f : s);
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
-}
-__device__ __forceinline__ float from_order_bits(uint32_t o) {
-  return __uint_as_float((o & 0x80000000u) ? (o & 0x7fffffffu) : ~o);
-}
-__device__ __forceinline__ uint64_t rank_key(float s, unsigned id) {
-  return isnan(s) ? 0ull : (uint64_t(order_bits(s)) << 32) | uint32_t(~id);
 }
 
 // Wave-wide maximum of an unsigned word (all 64 lanes active), uniform
@@ -39,115 +27,6 @@ __device__ __forceinline__ uint32_t wave_max_u32(uint32_t x) {
   x = max(x, uint32_t(__builtin_amdgcn_update_dpp(0, int(x), 0x142, 0xa, 0xf, false)));  // row_bcast:15
   x = max(x, uint32_t(__builtin_amdgcn_update_dpp(0, int(x), 0x143, 0xc, 0xf, false)));  // row_bcast:31
   return uint32_t(__builtin_amdgcn_readlane(int(x), 63));
-}
-
-// Wave-wide maximum of 64-bit keys: the high words first; the low words only
-// among the lanes that hold the highest high word.
-__device__ __forceinline__ uint64_t wave_max_key(uint64_t v) {
-  const uint32_t hi = uint32_t(v >> 32), lo = uint32_t(v);
-  const uint32_t mh = wave_max_u32(hi);
-  const uint64_t at = __ballot(hi == mh);
-  uint32_t ml;
-  if (__popcll(at) == 1)
-    ml = uint32_t(__builtin_amdgcn_readlane(int(lo), __ffsll(static_cast<long long>(at)) - 1));
-  else
-    ml = wave_max_u32(hi == mh ? lo : 0u);
-  return (uint64_t(mh) << 32) | ml;
-}
-
-// k rounds over J candidate keys per lane: each takes the wave-wide best key
-// below the previous pick; keys at or below `floor` are never picked.
-template <int J>
-__device__ __forceinline__ void rank_rounds(const uint64_t (&c)[J], int k, uint64_t *out, uint64_t floor) {
-  uint64_t prev = ~0ull;
-  for (int rank = 0; rank < k; ++rank) {
-    uint64_t b = 0ull;
-#pragma unroll
-    for (int i = 0; i < J; ++i) {
-      const uint64_t v = c[i] < prev ? c[i] : 0ull;
-      b = v > b ? v : b;
-    }
-    uint64_t best = wave_max_key(b);
-    if (best < floor) best = floor;
-    if ((threadIdx.x & 63) == 0) out[rank] = best;
-    prev = best;
-  }
-}
-
-// Keys that are ranked by counting; more (ties, flat logits) are first cut to
-// each wave's own top-k by k rounds of the wave-wide maximum.  Counting costs
-// count x ceil(count / 256) LDS reads: 512 are about as long as 64 rounds.
-constexpr int kSampleCap = 512;
-struct SampleShared {
-  uint64_t cand[kSampleCap];
-  uint32_t t[4];
-  int count;
-};
-
-// The workgroup's ranked top-k (k <= 64) of its 4096 keys (16 per lane) above
-// `floor`, which fills the ranks that no key took: put(rank, key) for every rank below k, from one thread each.
-template <typename Put>
-__device__ __forceinline__ void group_topk(const uint64_t (&key)[kSamplePerThread], int k, SampleShared &sh, uint64_t floor, Put put) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  // The largest t with at least k half-lane maxima whose score bits reach it
-  // (0: fewer than k): every key of the wave's top-k reaches t, and every key
-  // of the workgroup's top-k reaches each wave's t.
-  uint32_t hm0 = 0, hm1 = 0;
-#pragma unroll
-  for (int i = 0; i < kSamplePerThread; ++i) {
-    const uint32_t h = uint32_t(key[i] >> 32);
-    if (i < kSamplePerThread / 2) hm0 = max(hm0, h);
-    else hm1 = max(hm1, h);
-  }
-  uint32_t t = 0;
-#pragma unroll 1
-  for (int bit = 31; bit >= 0; --bit) {
-    const uint32_t c = t | (1u << bit);
-    if (__popcll(__ballot(hm0 >= c)) + __popcll(__ballot(hm1 >= c)) >= k) t = c;
-  }
-  if (lane == 0) sh.t[wave] = t;
-  if (tid == 0) sh.count = 0;
-  __syncthreads();
-  t = max(max(sh.t[0], sh.t[1]), max(sh.t[2], sh.t[3]));
-  uint32_t keep = 0;
-  int mine = 0;
-#pragma unroll
-  for (int i = 0; i < kSamplePerThread; ++i) {
-    const bool in = key[i] > floor && uint32_t(key[i] >> 32) >= t;
-    keep |= uint32_t(in) << i;
-    mine += __popcll(__ballot(in));
-  }
-  int base = 0;
-  if (lane == 0) base = atomicAdd(&sh.count, mine);
-  base = __builtin_amdgcn_readfirstlane(base);
-  if (base + mine <= kSampleCap) {
-#pragma unroll
-    for (int i = 0; i < kSamplePerThread; ++i) {
-      const bool in = (keep >> i) & 1u;
-      const uint64_t mask = __ballot(in);
-      if (in) sh.cand[base + __popcll(mask & ((1ull << lane) - 1ull))] = key[i];
-      base += __popcll(mask);
-    }
-  }
-  __syncthreads();
-  int count = sh.count, above = count;
-  if (count > kSampleCap) {  // the same in every thread
-    __syncthreads();
-    rank_rounds<kSamplePerThread>(key, k, sh.cand + wave * k, floor);
-    count = 4 * k;
-    __syncthreads();
-    above = 0;  // the lists end in floors
-    for (int j = 0; j < count; ++j) above += sh.cand[j] > floor;
-  }
-  for (int c = tid; c < count; c += kSampleThreads) {
-    const uint64_t v = sh.cand[c];
-    int rank = 0;
-#pragma unroll 8
-    for (int j = 0; j < count; ++j) rank += sh.cand[j] > v;
-    if (rank < k && v > floor) put(rank, v);  // keys above the floor are distinct
-  }
-  if (tid < k && tid >= above) put(tid, floor);  // ranks that no key took
-  __syncthreads();
 }
 
 }  // namespace dev
