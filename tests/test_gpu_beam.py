@@ -334,6 +334,67 @@ def test_beam_search(ctx, rng, graph):
          *t2.values())
 
 
+def test_beam_search_with_ends(ctx, rng):
+    """Beams that end stay on the device too: the next step's `done` is a gather of a table with a one at the end token, by
+    the selected tokens.  Every step equals a search without any cache, in which an ended beam is carried on as it is."""
+    m, page, beams, steps, prompts, end = Model(rng), 32, 4, 14, [[int(x) for x in rng.integers(0, 211, n)] for n in (9, 21)], 45
+    groups, width, pwidth = len(prompts), 1, 1
+    n = groups * beams
+    order = rng.permutation(n * width + groups * pwidth).astype(np.int32)
+    caches = [Store(rng, F32, order.size, page, m.kv, m.dim).put(ctx) for _ in range(m.layers)]
+    total, lengths = sum(map(len, prompts)), [len(p) for p in prompts]
+    ptables, plengths = words(ctx, order[n * width:]), words(ctx, lengths)
+    starts = words(ctx, np.cumsum([0] + lengths))
+    prefill = hip.PagedBatch(ptables, plengths, groups, total, pwidth, starts=starts)
+    t, ids = m.tensors(ctx, total), words(ctx, sum(prompts, []))
+    m.forward(ctx, t, prefill, caches, ids, total)
+    start = ctx.Download(t["logits"]).reshape(total, -1)[np.cumsum(lengths) - 1]
+    t2, logits = m.tensors(ctx, n), up(ctx, np.repeat(start, beams, 0).astype(np.float32))
+    ctx.Copy(t2["logits"], logits, n * m.vocab)
+    tab, blen = [words(ctx, order[:n * width]), ctx.NewTensor(n * width)], words(ctx, [0] * n)
+    batches = [hip.PagedBatch(x, blen, n, n, width, prefix_tables=ptables, prefix_lengths=plengths, prefix_pages=pwidth,
+                              share=beams) for x in tab]
+    scores = up(ctx, np.where(np.arange(n) % beams == 0, np.float32(0), np.float32(-np.inf)))
+    best, parents, tokens = (ctx.NewTensor(n) for _ in range(3))
+    ends, done = words(ctx, np.arange(m.vocab) == end), words(ctx, [0] * n)
+    texts = [[list(p) for _ in range(beams)] for p in prompts]
+    sums = [[0.0] + [-np.inf] * (beams - 1) for _ in prompts]
+    over = [[False] * beams for _ in prompts]
+    for i in range(steps):
+        ctx.BeamSelect(parents, tokens, best, t2["logits"], scores, done, groups, beams, m.vocab, beams, end)
+        ctx.Copy(scores, best, n)
+        ctx.GatherRows(done, ends, tokens, n, 1)
+        ctx.PagedReorder(batches[i % 2], tab[(i + 1) % 2], parents, caches)
+        ctx.PagedAdvance(batches[(i + 1) % 2], page)
+        m.forward(ctx, t2, batches[(i + 1) % 2], caches, tokens, n)
+        got = [ctx.Download(x, dtype=d).reshape(groups, beams) for x, d in ((parents, np.int32), (tokens, np.int32),
+                                                                            (best, np.float32), (done, np.int32))]
+        for g in range(groups):
+            top, value = ended_step(m, texts[g], sums[g], over[g], end)
+            texts[g] = [texts[g][o // m.vocab] + [int(o % m.vocab)] for o in top]
+            sums[g], over[g] = value.tolist(), [int(o % m.vocab) == end for o in top]
+            assert (got[0][g] - g * beams).tolist() == (top // m.vocab).tolist(), (i, g)
+            assert got[1][g].tolist() == (top % m.vocab).tolist(), (i, g)
+            assert np.max(np.abs(got[2][g] - value)) <= 1e-4 * max(1.0, np.max(np.abs(value)))
+            assert got[3][g].tolist() == [int(x) for x in over[g]]
+    assert any(map(any, over)) and not all(map(all, over))
+    free(ctx, ptables, plengths, starts, ids, blen, scores, best, parents, tokens, logits, ends, done, *tab, *caches,
+         *t.values(), *t2.values())
+
+
+def ended_step(m, texts, sums, over, end):
+    """One group's step in 64 bits: candidates in order and their scores; an ended beam only offers `end` at its score."""
+    x = np.stack([m.logits(text) for text in texts])
+    x -= x.max(1, keepdims=True)
+    cand = np.array(sums)[:, None] + x - np.log(np.exp(x).sum(1, keepdims=True))
+    for b, o in enumerate(over):
+        if o:
+            cand[b] = -np.inf
+            cand[b, end] = sums[b]
+    top = np.argsort(-cand.reshape(-1), kind="stable")[:len(texts)]
+    return top, cand.reshape(-1)[top]
+
+
 def test_two_graphs_and_a_larger_call(ctx, rng):
     """Two captured graphs share the context's workspace; a larger eager call between their replays outgrows it."""
     from tests.test_gpu_paged import Batch

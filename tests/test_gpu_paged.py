@@ -433,6 +433,22 @@ def test_attention_repeats_and_ignores_the_batch(ctx, rng):
     assert np.array_equal(a, run_attention(ctx, store, batch, q, 32, force_starts=True))
 
 
+@pytest.mark.parametrize("n,own,prefix,share", [([1] * 5, [700, 3, 64, 1000, 129], None, 1),
+                                                ([40, 1, 9], [200, 50, 9], None, 1),
+                                                ([1] * 6, [20, 90, 7, 33, 8, 64], [300, 41], 3)])
+def test_attention_of_a_sequence_among_others(ctx, rng, n, own, prefix, share):
+    """What the other sequences' keys, values and queries are makes no difference to a sequence, to the bit."""
+    page, kv, heads, dim = 64, 2, 8, 128
+    batch = Batch(rng, page, n, own, prefix, share)
+    store, other = (Store(rng, BF16, batch.pages, page, kv, dim) for _ in range(2))
+    q, q2 = (rng.standard_normal((batch.rows, heads, dim)).astype(np.float32) for _ in range(2))
+    mine = np.concatenate([batch.tables[0]] + ([batch.prefix_tables[0]] if prefix else []))
+    other.x[mine] = store.x[mine]
+    q2[:n[0]] = q[:n[0]]
+    a, b = run_attention(ctx, store, batch, q, heads), run_attention(ctx, other, batch, q2, heads)
+    assert np.array_equal(a[:n[0]], b[:n[0]]) and not np.any(np.all(a[n[0]:] == b[n[0]:], axis=(1, 2)))
+
+
 def test_attention_in_a_cache_past_32_bit_offsets(ctx, rng):
     """Pages whose byte offsets pass 2^32 (a tensor holds up to 2^31 words)."""
     page, kv, heads, dim = 256, 8, 16, 256
