@@ -53,9 +53,11 @@ struct qnn_ctx_s {
   size_t partial_floats = 0;
   unsigned *counters = nullptr;
   size_t counter_count = 0;
+  bool splitk_captured = false;  // a graph may hold its addresses
   // generic workspace (MoE plan and hidden states, activation quantisation)
   void *work = nullptr;
   size_t work_bytes = 0;
+  bool work_captured = false;
   std::vector<void *> retired;  // outgrown workspaces that captured graphs still write to
   // upload staging
   void *staging = nullptr;
@@ -270,22 +272,26 @@ qnn_tensor_s *new_tensor(qnn_ctx_s *ctx, int count) {
 }
 
 // ---------------------------------------------------------------- workspace
-// An outgrown workspace.  A captured graph keeps the addresses it was captured
-// with, so once there is a graph the memory stays until the context goes.
-void retire(qnn_ctx_s *ctx, void *p) {
+// An outgrown workspace.  A graph keeps the addresses it was captured with, so
+// memory that a call took while capturing stays until the context goes.
+void retire(qnn_ctx_s *ctx, void *p, bool captured) {
   if (!p) return;
-  if (ctx->graphs.empty()) (void)hipFree(p);
-  else ctx->retired.push_back(p);
+  if (captured) ctx->retired.push_back(p);
+  else (void)hipFree(p);
 }
 
 void ensure_splitk(qnn_ctx_s *ctx, size_t partial_floats, size_t counters) {
-  if (partial_floats <= ctx->partial_floats && counters <= ctx->counter_count) return;
+  if (partial_floats <= ctx->partial_floats && counters <= ctx->counter_count) {
+    ctx->splitk_captured |= ctx->capturing;
+    return;
+  }
   if (ctx->capturing) fail(QNN_E_INVALID_OP, "split-K workspace growth during graph capture (run the sequence once first)");
   sync(ctx);
   partial_floats = std::max(partial_floats, ctx->partial_floats);
   counters = std::max(counters, ctx->counter_count);
-  retire(ctx, ctx->partial);
-  retire(ctx, ctx->counters);
+  retire(ctx, ctx->partial, ctx->splitk_captured);
+  retire(ctx, ctx->counters, ctx->splitk_captured);
+  ctx->splitk_captured = false;
   ctx->partial = nullptr;
   ctx->counters = nullptr;
   ctx->partial_floats = ctx->counter_count = 0;  // until both are there again
@@ -305,10 +311,14 @@ void ensure_splitk(qnn_ctx_s *ctx, size_t partial_floats, size_t counters) {
 }
 
 void *ensure_work(qnn_ctx_s *ctx, size_t bytes) {
-  if (bytes <= ctx->work_bytes) return ctx->work;
+  if (bytes <= ctx->work_bytes) {
+    ctx->work_captured |= ctx->capturing;
+    return ctx->work;
+  }
   if (ctx->capturing) fail(QNN_E_INVALID_OP, "workspace growth during graph capture (run the sequence once first)");
   sync(ctx);
-  retire(ctx, ctx->work);
+  retire(ctx, ctx->work, ctx->work_captured);
+  ctx->work_captured = false;
   ctx->work = nullptr;
   ctx->work_bytes = 0;
   hip_check(hipMalloc(&ctx->work, bytes), "workspace allocation");

@@ -205,3 +205,38 @@ assert cache._c.page_count == 5
 ctx.PagedAttention(out, q, other, batch, 1)
 ctx.Flush()
 """)
+
+
+def test_outgrown_workspaces_that_no_graph_uses_are_freed(host):
+    """A workspace outlives its growth only if a graph was captured with it, not because there is a graph."""
+    host(GROW + """
+logits, scores, found = ctx.NewTensor(64 << 20), ctx.NewTensor(1), [ctx.NewTensor(4) for _ in range(3)]
+def select(vocab):
+    ctx.BeamSelect(*found, logits, scores, None, 1, 1, vocab, 4)
+select(1 << 20)
+before = rec.rec_live_bytes()
+ctx.GraphBegin()
+select(1 << 20)
+graph = ctx.GraphEnd()
+for i in range(2, 64):
+    select(i << 20)
+grown = 63 << 13
+assert rec.rec_live_bytes() == before + grown, (rec.rec_live_bytes() - before, grown)  # the graph's, and the last
+ctx.GraphLaunch(graph)
+before = rec.rec_live_bytes()
+linear(large, 9728, 4096)  # outgrows the split-K workspace, which no graph has
+assert rec.rec_live_bytes() > before
+ctx.GraphBegin()
+linear(large, 9728, 4096)
+ctx.GraphEnd()
+kept = rec.rec_live_bytes()
+larger = int4(9728, 9728)
+y = ctx.NewTensor(9728)
+middle = rec.rec_live_bytes()
+linear(larger, 9728, 9728)
+linear(small, 4096, 64)
+assert rec.rec_live_bytes() > middle
+ctx.Recycle(found[0])
+ctx.close()
+assert rec.rec_live_bytes() == 0
+""")
