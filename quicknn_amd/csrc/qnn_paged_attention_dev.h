@@ -78,6 +78,7 @@ struct Args {
   int cols[2];                       // columns of a part
   float *whole;                      // of whole items (with prefixes), [own, prefix][KV head][rows x group][dim + 4]
   int prefix_tiles;                  // id of the first wide tile of the prefixes
+  int *first_keys;                   // per group: the first prefix key that any row sees (with prefixes and a window)
 };
 
 __device__ __forceinline__ int row_sequence(const PagedBatch &b, int row) {
@@ -122,15 +123,7 @@ __device__ __forceinline__ Owner owner_of(const Args &g, int o) {
     w.end = max(w.first, dev::first_row(b, (p + 1) * b.share));
     w.keys = w.prefix = dev::prefix_length<REPORT>(b, p);
     w.table = b.prefix_tables + size_t(p) * b.prefix_pages;
-    if (g.a.window > 0 && w.keys > 0) {
-      int at = 0x3fffffff;
-      for (int s = p * b.share; s < (p + 1) * b.share; ++s) {
-        int first, end;
-        dev::row_range<false>(b, s, first, end);
-        if (end > first) at = min(at, dev::own_length<false>(b, s) - (end - first));
-      }
-      w.low = max(0, w.prefix + at - g.a.window + 1);
-    }
+    if (g.a.window > 0 && w.keys > 0) w.low = g.first_keys[p];
   }
   w.cols = (w.end - w.first) * g.group;
   return w;
@@ -1489,6 +1482,7 @@ Plan plan_of(const PagedAttn &a, uint8_t *ws) {
     g.parts[c] = reinterpret_cast<float *>(take(slots * g.cols[c] * (a.c.dim + 4) * 4));
   }
   g.whole = reinterpret_cast<float *>(take(groups ? int64_t(2) * b.rows * a.heads * (a.c.dim + 4) * 4 : 0));
+  g.first_keys = reinterpret_cast<int *>(take(groups && a.window > 0 ? groups * 4 : 0));
   p.bytes = at;
   return p;
 }

@@ -433,6 +433,34 @@ def test_attention_repeats_and_ignores_the_batch(ctx, rng):
     assert np.array_equal(a, run_attention(ctx, store, batch, q, 32, force_starts=True))
 
 
+def test_attention_of_a_large_group_with_a_window(ctx, rng):
+    """A window over a prefix that many sequences share hides keys; it shall not cost a look at the whole group for every
+    row and head.  At 2000 sequences that was more than twenty times the time without a window."""
+    count, page, kv, heads, dim = 2000, 32, 2, 8, 64
+    n = [int(x) for x in rng.integers(0, 3, count)]
+    store = Store(rng, BF16, 60, page, kv, dim)
+    batch = Batch.__new__(Batch)
+    batch.n, batch.own, batch.share, batch.page = n, [x + int(y) for x, y in zip(n, rng.integers(0, 50, count))], count, page
+    batch.tables, batch.prefix_tables = (rng.integers(0, 60, s).astype(np.int32) for s in ((count, 2), (1, 20)))
+    batch.has_prefix, batch.prefix = True, [600]
+    batch.starts = np.concatenate([[0], np.cumsum(n)]).astype(np.int32)
+    batch.rows = int(batch.starts[-1])
+    q = rng.standard_normal((batch.rows, heads, dim)).astype(np.float32)
+    cache, b, tq, dst, times = store.put(ctx), batch.put(ctx), up(ctx, q), ctx.NewTensor(q.size), {}
+    for window in (0, 300):
+        want, took = attention(store, batch, q, heads, window), []
+        for _ in range(6):
+            ctx.EventRecord(0)
+            ctx.PagedAttention(dst, tq, cache, b, heads, window)
+            ctx.EventRecord(1)
+            ctx.Flush()
+            took.append(ctx.EventElapsedMs(0, 1))
+        times[window] = min(took)
+        assert np.max(np.abs(ctx.Download(dst).reshape(q.shape) - want)) <= tol(dim) * np.max(np.abs(want))
+    assert times[300] <= 4 * times[0], times
+    free(ctx, cache, b, tq, dst)
+
+
 @pytest.mark.parametrize("n,own,prefix,share", [([1] * 5, [700, 3, 64, 1000, 129], None, 1),
                                                 ([40, 1, 9], [200, 50, 9], None, 1),
                                                 ([1] * 6, [20, 90, 7, 33, 8, 64], [300, 41], 3)])
