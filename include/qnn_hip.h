@@ -418,17 +418,24 @@ int qnn_moe_experts(qnn_ctx *ctx, qnn_expert_set *set, qnn_tensor *dst, qnn_tens
  * A decode step of a beam search, without a host round trip:
  *   qnn_beam_select     best continuations of the last logits
  *   qnn_paged_reorder   tables and partial pages follow the parents
- *   qnn_gather_rows     so do dense states (token histories, seen flags)
+ *   qnn_gather_rows     so do dense states (token histories, seen flags), and the
+ *                       next step's `done` is gathered by the selected tokens
+ *                       from a table of words with a one at end_token
  *   qnn_paged_advance   lengths grow by the rows of this step
  *   per layer: projections, qnn_paged_append, qnn_paged_attention, MLP
  * All batch data are words in tensors, so that a captured graph can be replayed
  * while lengths and tables change.
  *
+ * That loop takes as many continuations as there are beams.  Of more (select >
+ * beams) the caller chooses which go on, and makes parents, tokens and scores
+ * of them.
+ *
  * Batch data are checked on the device: a length past its table, a row start
- * that does not ascend or passes `rows`, a page id outside the cache, a parent
- * outside its group or a row index outside its source never leads to an access
- * out of range; the next qnn_download fails with QNN_E_INVALID_OP, and what the
- * call wrote for the rows concerned is unspecified.
+ * that does not ascend or passes `rows`, a page id outside the cache where a
+ * call reads or writes that page, a parent outside its group or a row index
+ * outside its source never leads to an access out of range; the next
+ * qnn_download fails with QNN_E_INVALID_OP, and what the call wrote for the rows
+ * concerned is unspecified.
  * ------------------------------------------------------------------------- */
 /* The KV cache of one layer: page_count pages of page_size tokens (32, 64, 128
  * or 256), in one tensor of 2 * page_count * kv_heads * page_size * dim
@@ -438,7 +445,8 @@ int qnn_moe_experts(qnn_ctx *ctx, qnn_expert_set *set, qnn_tensor *dst, qnn_tens
  *   keys          blocks of 16 tokens, [dim / E][16 tokens][E channels]
  *   values, BF16  groups of 32 tokens, [4][dim][8 tokens]: token 16 a + 4 g + b
  *                 of the group (a < 2, g < 4, b < 4) at [g][.][4 a + b]
- *   values, F32   blocks of 16 tokens, [4][dim][4 tokens]: token 4 g + b at [g][.][b] */
+ *   values, F32   blocks of 16 tokens, [4][dim][4 tokens]: token 4 g + b at [g][.][b]
+ * Up to 1024 KV heads (and 65535 query heads). */
 typedef struct {
   qnn_tensor *pages;
   int32_t dtype;      /* QNN_DT_F32 or QNN_DT_BF16 */
@@ -457,6 +465,7 @@ typedef struct {
  * [sequences / share][prefix_pages] and prefix_lengths [sequences / share],
  * both NULL without.  Row i of n of a sequence has own position
  * length - n + i, and absolute position prefix length + own position.
+ * Up to 65535 sequences and rows, tables and prefix tables of up to 2^30 tokens.
  * A call's result is none of these tensors (but the lengths of
  * qnn_paged_advance, which are no other one of them). */
 typedef struct {
@@ -467,7 +476,9 @@ typedef struct {
 /* Appends keys and values: k, v [rows][kv_heads][dim].  k (and q
  * [rows][heads][dim] into q_out, which may be q; both may be NULL) is rotated by
  * its absolute position as QNN_GO_LLM_ROPE does, with theta = 0 not at all; a
- * BF16 cache holds the rounded values (to nearest even). */
+ * BF16 cache holds the rounded values (to nearest even).  Calls of two rows per
+ * sequence and more step from angle to angle in 64 bits: a rounding may then,
+ * rarely, go the other way. */
 int qnn_paged_append(qnn_ctx *ctx, const qnn_paged_cache *cache, const qnn_paged_batch *batch, qnn_tensor *k,
                      qnn_tensor *v, qnn_tensor *q, qnn_tensor *q_out, int heads, float theta);
 /* lengths[s] += rows of sequence s, up to what table_pages pages of page_size tokens hold. */
@@ -476,8 +487,8 @@ int qnn_paged_advance(qnn_ctx *ctx, const qnn_paged_batch *batch, int page_size)
  * own keys up to its position, the last `window` of them when window > 0;
  * scores scaled by `scale` (0: 1/sqrt(dim)) and capped as by
  * qnn_cached_attention.  heads / kv_heads query heads per KV head; q, dst:
- * [rows][heads][dim].  A prefix's keys are read once for all rows of its
- * group.  A row that sees no key, or whose scores are all minus infinity, gets
+ * [rows][heads][dim].  A prefix's keys are read once for every 128 columns (rows
+ * times query heads per KV head) of its group.  A row that sees no key, or whose scores are all minus infinity, gets
  * zeros; keys that a row does not see (and what is behind a sequence's last
  * key) do not reach it, infinite or NaN as they may be.  A row may lie in front
  * of its sequence's own keys (length below its rows): it sees the prefix up to

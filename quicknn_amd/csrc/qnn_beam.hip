@@ -10,9 +10,11 @@
 // ranked by counting.  The tile is chosen small enough that a group has several
 // times `select` of them, down to a wave's width.  Where more than 512 reach T
 // (ties: flat logits, or logits masked with a large finite value, all of which
-// round to one fp32 candidate), every wave keeps its best in order in one more
+// round to one fp32 candidate; or `select` near 64, where the bound behind T is
+// the least of a wave's maxima), every wave keeps its best in order in one more
 // pass, and their lists are ranked: 8 groups of 8 beams over 151936 masked
-// tokens, 16 selected, 490 us (11.4 ms with a pass over all of them per rank).
+// tokens, 16 selected, 490 us; 4 groups of 32 beams over 32000, 64 selected, 600
+// us (11.4 and 25 ms with a pass over all of them per rank).
 //
 // Candidates are compared in 64 bits.  Logits of one beam are exact there; two
 // beams' normalisers carry the roundings of fp32 sums, so the order across
@@ -20,7 +22,7 @@
 // give equal sums, whatever their rows' alignment.  The scores are rounded to
 // fp32 once.
 //
-// What bounds it: the first launch memory (38.9 MB of logits in 7.5 us), the
+// What bounds it: the first launch memory (38.9 MB of logits in 8 us), the
 // second one chain of latencies in one workgroup per group (12 us for 8 groups
 // of 8 beams over 151936 tokens, select 16; 8 us for 4 beams over 32000).  A
 // ranked list per 4096-token tile in the first launch and a merge of the lists

@@ -10,12 +10,13 @@
 //
 // Columns.  The rows of a sequence times the query heads of a KV head are the
 // columns that read the same keys; so are the rows of all sequences of a group
-// for the prefix, whose keys are read once for all of them.  Both products run
-// on the matrix cores transposed, S^T = K Q^T and O^T = V^T P^T, 32 columns by
-// 32 keys: a lane's results then belong to one column, its running maximum,
-// sum and rescaling are in-lane (one exchange of the two half-waves), and the
-// weights are, as they stand in its registers, the operand of the second
-// product.  Pages hold K and V in operand order, so nothing is rearranged.
+// for the prefix, whose keys are read once for each tile of up to 128 of them.
+// Both products run on the matrix cores transposed, S^T = K Q^T and O^T = V^T
+// P^T, 32 columns by 32 keys: a lane's results then belong to one column, its
+// running maximum, sum and rescaling are in-lane (one exchange of the two
+// half-waves), and the weights are, as they stand in its registers, the operand
+// of the second product.  Pages hold K and V in operand order, so nothing is
+// rearranged.
 //
 // Arithmetic.  A BF16 cache multiplies on v_mfma_f32_32x32x16_bf16, three
 // products each: q and the weights are split into three bf16 planes by
@@ -35,10 +36,10 @@
 //
 // What bounds it (32 query heads on 8, 128 channels, BF16, per call).  Single
 // tokens: memory, forty sequences up to 8k keys (736 MB) 124 us, 6.3 TB/s in the
-// main kernel, matrix cores 14 % busy; one token at 4k keys 16 us, a chain of
+// main kernel, matrix cores 14 % busy; one token at 4k keys 15 us, a chain of
 // latencies (share 3 us, table, K, V, join of the waves, second launch).  Many
 // columns: the matrix cores with their three products, 1000 rows over 8000 keys
-// 350 us (369 GFLOP of products, 1.05 PFLOP/s; a large library product reaches
+// 343 us (369 GFLOP of products, 1.08 PFLOP/s; a large library product reaches
 // 1.14 on this card).
 //
 // Infinities and NaN.  A plane or weight of zero times an infinity would be
