@@ -519,7 +519,10 @@ int qnn_gather_rows(qnn_ctx *ctx, qnn_tensor *dst, qnn_tensor *src, qnn_tensor *
  * of logits.  done (words, may be NULL) != 0: the beam's only candidate is
  * end_token at the beam's own score; its other tokens, and all of a beam whose
  * score is not finite or whose logits hold a NaN, plus infinity or nothing
- * finite, are at minus infinity (and follow in order of b, v). */
+ * finite, are at minus infinity (and follow in order of b, v).  Candidates are
+ * compared in 64 bits, but two beams' sums of exponentials carry roundings of
+ * about 1e-7: candidates of different beams that are closer than that may change
+ * places, unless the beams' logits are the same. */
 int qnn_beam_select(qnn_ctx *ctx, qnn_tensor *parents, qnn_tensor *tokens, qnn_tensor *best, qnn_tensor *logits,
                     qnn_tensor *scores, qnn_tensor *done, int groups, int beams, int vocab, int select, int end_token);
 
